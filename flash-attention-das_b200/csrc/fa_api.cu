@@ -132,10 +132,10 @@ int* stream_tickets(cudaStream_t stream, int64_t count) {
 
 int elem_size(int dtype) { return dtype == FA_B200_E4M3 ? 1 : 2; }
 
-// 4-D tile descriptor over (d, heads, rows, batch) with a 128-byte-swizzled box of (128 bytes, 1, box_rows, 1).
+// 4-D tile descriptor over (d, heads, rows, batch) with a 128-byte-swizzled box of (128 bytes, box_heads, box_rows, 1).
 // Strides are in elements.  Out-of-range rows read as zero.
 int make_tmap(CUtensorMap* out, const void* base, int dtype, int64_t heads, int64_t rows, int64_t batch,
-              int64_t head_stride, int64_t row_stride, int64_t batch_stride, int box_rows, int d = kHeadDim) {
+              int64_t head_stride, int64_t row_stride, int64_t batch_stride, int box_rows, int d = kHeadDim, int box_heads = 1) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) { set_error("cuTensorMapEncodeTiled", "driver entry point not found"); return FA_B200_ERR_CUDA; }
   const int es = elem_size(dtype);
@@ -145,7 +145,7 @@ int make_tmap(CUtensorMap* out, const void* base, int dtype, int64_t heads, int6
                         static_cast<cuuint64_t>(rows > 0 ? rows : 1), static_cast<cuuint64_t>(batch > 0 ? batch : 1)};
   auto fix = [&](int64_t s) { return static_cast<cuuint64_t>((s > 0 ? s : d) * es); };
   cuuint64_t strides[3] = {fix(head_stride), fix(row_stride), fix(batch_stride)};
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), 1u, static_cast<cuuint32_t>(box_rows), 1u};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows), 1u};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUtensorMapDataType dt = dtype == FA_B200_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                            : dtype == FA_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -535,6 +535,7 @@ int fa_b200_combine(const fa_b200_combine_params* p, void* stream) {
   k.out_scale = p->out_scale;
   k.s_aux = p->s_aux;
   k.s_aux_dtype = p->s_aux_dtype;
+  k.group = 1;
   k.d = p->d;
   k.o_part_stride = p->o_part_stride > 0 ? p->o_part_stride : static_cast<int64_t>(p->rows) * p->d;
   k.lse_part_stride = p->lse_part_stride > 0 ? p->lse_part_stride : p->rows;
@@ -633,10 +634,29 @@ int fa_b200_exchange_combine(const fa_b200_exchange_params* p, void* stream) {
   return FA_B200_OK;
 }
 
-int fa_b200_decode_paged(const fa_b200_decode_params* p, void* stream_) {
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+// Scores of a decode that accumulates token weights: [b][h_k][rows][stride] fp32 behind the split-KV partials.
+static int64_t score_stride(const DecodePlan& pl) { return (static_cast<int64_t>(pl.max_len) + 127) / 128 * 128; }
+static size_t score_ws_bytes(const fa_b200_decode_params* p, const DecodePlan& pl) {
+  const size_t sq = p->seqlen_q > 1 ? p->seqlen_q : 1;
+  return static_cast<size_t>(p->b) * p->h * sq * score_stride(pl) * sizeof(float);
+}
+static size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// e: page lists per kv head and / or token weights (fa_b200_decode_budget); nullptr: plain decode.
+static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_budget_params* e_, cudaStream_t stream) {
   DecodePlan pl = plan_decode(p);
   if (pl.status != FA_B200_OK) return pl.status;
+  const bool per_head = e_ && e_->per_kv_head;
+  const bool weights = e_ && e_->weights_out;
+  if (weights) {
+    if (per_head || p->o_partial_out || p->v_transposed) return FA_B200_ERR_UNSUPPORTED;
+    if (!p->softmax_lse) return FA_B200_ERR_NULL;
+    if (e_->weights_capacity < 0) return FA_B200_ERR_SHAPE;
+    if (e_->weights_in_batch_stride < 0 || e_->weights_in_head_stride < 0 || e_->weights_out_batch_stride < 0 ||
+        e_->weights_out_head_stride < 0)
+      return FA_B200_ERR_STRIDE;
+  }
+  if (per_head && e_->block_table_head_stride < 0) return FA_B200_ERR_STRIDE;
   if (!p->q || !p->k_cache || !p->v_cache || !p->block_table || !p->cache_seqlens) return FA_B200_ERR_NULL;
   if (!p->out && !p->o_partial_out) return FA_B200_ERR_NULL;
   if (p->o_partial_out && !p->lse_partial_out) return FA_B200_ERR_NULL;
@@ -654,7 +674,8 @@ int fa_b200_decode_paged(const fa_b200_decode_params* p, void* stream_) {
       (p->q_row_stride * qes) % q_piece != 0 || p->o_batch_stride % 8 != 0 || p->o_head_stride % 8 != 0)
     return FA_B200_ERR_STRIDE;
   if (p->b == 0) return FA_B200_OK;
-  const size_t need = decode_ws_bytes(p, pl);
+  const size_t part_bytes = decode_ws_bytes(p, pl);
+  const size_t need = weights ? align256(part_bytes) + score_ws_bytes(p, pl) : part_bytes;
   if (need > 0 && (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace))) return FA_B200_ERR_WORKSPACE;
 
   CUtensorMap tk, tv;
@@ -691,6 +712,13 @@ int fa_b200_decode_paged(const fa_b200_decode_params* p, void* stream_) {
   k.o_batch_stride = p->o_batch_stride;
   k.o_head_stride = p->o_head_stride;
   k.bt_stride = p->block_table_batch_stride;
+  k.bt_head_stride = per_head ? e_->block_table_head_stride : 0;
+  k.len_b = per_head ? p->h_k : 1;
+  k.len_h = per_head ? 1 : 0;
+  if (weights) {
+    k.scores = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + align256(part_bytes));
+    k.score_stride = score_stride(pl);
+  }
   k.b = p->b; k.h = p->h; k.h_k = p->h_k; k.group = pl.group;
   k.page_size = p->page_size;
   k.box_tok = pl.box_tok;
@@ -769,6 +797,9 @@ int fa_b200_decode_paged(const fa_b200_decode_params* p, void* stream_) {
     c.o_partial = k.o_partial;
     c.lse_partial = k.lse_partial;
     c.seqlens = p->cache_seqlens;
+    c.len_b = k.len_b;
+    c.len_h = k.len_h;
+    c.group = pl.group;
     c.parts_per_row = nullptr;
     c.num_parts = pl.num_partitions;
     c.rows = p->b * p->h * k.sq;
@@ -802,7 +833,46 @@ int fa_b200_decode_paged(const fa_b200_decode_params* p, void* stream_) {
     if (e != cudaSuccess) return cuda_fail("combine launch", e);
     g_launches++;
   }
+  if (weights) {
+    WeightsFinishParams w{};
+    w.scores = k.scores;
+    w.score_stride = k.score_stride;
+    w.lse = p->softmax_lse;
+    w.seqlens = p->cache_seqlens;
+    w.w_in = e_->weights_in;
+    w.w_out = e_->weights_out;
+    w.win_b = e_->weights_in_batch_stride; w.win_h = e_->weights_in_head_stride;
+    w.wout_b = e_->weights_out_batch_stride; w.wout_h = e_->weights_out_head_stride;
+    w.b = p->b; w.h = p->h; w.h_k = p->h_k; w.group = pl.group; w.sq = k.sq;
+    w.max_len = pl.max_len;
+    w.capacity = e_->weights_capacity;
+    w.causal = k.causal;
+    w.window_left = k.window_left;
+    w.decay = e_->decay;
+    w.dependent_launch = g_env.dependent_launch;
+    e = launch_weights_finish(w, stream);
+    if (e != cudaSuccess) return cuda_fail("token weights launch", e);
+    g_launches++;
+  }
   return FA_B200_OK;
+}
+
+int fa_b200_decode_paged(const fa_b200_decode_params* p, void* stream) {
+  return decode_paged(p, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int fa_b200_decode_budget(const fa_b200_decode_params* p, const fa_b200_decode_budget_params* e, void* stream) {
+  if (!p || !e) return FA_B200_ERR_NULL;
+  if (e->struct_size != sizeof(fa_b200_decode_budget_params)) return FA_B200_ERR_ABI;
+  return decode_paged(p, e, static_cast<cudaStream_t>(stream));
+}
+
+size_t fa_b200_decode_budget_workspace_bytes(const fa_b200_decode_params* p, const fa_b200_decode_budget_params* e) {
+  if (!e || e->struct_size != sizeof(fa_b200_decode_budget_params)) return 0;
+  DecodePlan pl = plan_decode(p);
+  if (pl.status != FA_B200_OK) return 0;
+  const size_t parts = decode_ws_bytes(p, pl);
+  return e->weights_out ? align256(parts) + score_ws_bytes(p, pl) : parts;
 }
 
 // ---- decode without caller-provided scratch ------------------------------------------------------
@@ -1034,6 +1104,227 @@ static int fwd_common(const fa_b200_fwd_params* p, void* stream_, bool sparse) {
 
 int fa_b200_fwd(const fa_b200_fwd_params* p, void* stream) { return fwd_common(p, stream, false); }
 int fa_b200_fwd_sparse(const fa_b200_fwd_params* p, void* stream) { return fwd_common(p, stream, true); }
+
+// ---- decode with a bounded cache --------------------------------------------------------------------
+static bool budget_page_ok(int page) { return page == 16 || page == 32 || (page >= 64 && page % 64 == 0); }
+
+int fa_b200_page_bounds(const fa_b200_page_bounds_params* p, void* stream) {
+  if (!p) return FA_B200_ERR_NULL;
+  if (p->struct_size != sizeof(fa_b200_page_bounds_params)) return FA_B200_ERR_ABI;
+  if (!head_dim_ok(p->d, false)) return FA_B200_ERR_HEADDIM;
+  const bool fp8 = p->dtype == FA_B200_E4M3 || p->dtype == FA_B200_E5M2;
+  if (!fp8 && p->dtype != FA_B200_F16 && p->dtype != FA_B200_BF16) return FA_B200_ERR_DTYPE;
+  if (fp8 ? (p->bounds_dtype != FA_B200_F16 && p->bounds_dtype != FA_B200_BF16) : p->bounds_dtype != p->dtype) return FA_B200_ERR_DTYPE;
+  if (p->b < 0 || p->h_k <= 0 || p->num_blocks < 0 || p->max_blocks_per_seq < 0 || p->new_tokens < 0) return FA_B200_ERR_SHAPE;
+  if (!budget_page_ok(p->page_size)) return FA_B200_ERR_PAGE;
+  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > (1ll << 30)) return FA_B200_ERR_TOO_LARGE;
+  if (p->b == 0 || p->max_blocks_per_seq == 0 || p->num_blocks == 0) return FA_B200_OK;
+  if (!p->k_cache || !p->page_bounds || !p->block_table || !p->cache_seqlens) return FA_B200_ERR_NULL;
+  const int es = fp8 ? 1 : 2;
+  if (!aligned16(p->k_cache) || !aligned16(p->page_bounds)) return FA_B200_ERR_ALIGN;
+  if (!stride_ok(p->k_block_stride, es) || !stride_ok(p->k_row_stride, es) || !stride_ok(p->k_head_stride, es)) return FA_B200_ERR_STRIDE;
+  PageBoundsParams k{};
+  k.status = status_ptr();
+  if (!k.status) return cuda_fail("status word", cudaGetLastError());
+  k.k_cache = p->k_cache;
+  k.k_blk = p->k_block_stride; k.k_row = p->k_row_stride; k.k_h = p->k_head_stride;
+  k.bounds = p->page_bounds;
+  k.block_table = p->block_table;
+  k.bt_stride = p->block_table_batch_stride;
+  k.seqlens = p->cache_seqlens;
+  k.b = p->b; k.h_k = p->h_k; k.d = p->d;
+  k.page_size = p->page_size; k.num_blocks = p->num_blocks; k.max_blocks = p->max_blocks_per_seq;
+  k.new_tokens = p->new_tokens;
+  // n consecutive tokens lie in at most (n - 1) / page + 2 pages
+  k.slots = p->max_blocks_per_seq;
+  if (p->new_tokens > 0 && (p->new_tokens - 1) / p->page_size + 2 < k.slots) k.slots = (p->new_tokens - 1) / p->page_size + 2;
+  const cudaError_t e = launch_page_bounds(p->dtype, p->bounds_dtype, k, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("page bounds launch", e);
+  g_launches++;
+  return FA_B200_OK;
+}
+
+static int page_select_status(const fa_b200_page_select_params* p) {
+  if (!p) return FA_B200_ERR_NULL;
+  if (p->struct_size != sizeof(fa_b200_page_select_params)) return FA_B200_ERR_ABI;
+  if (!head_dim_ok(p->d, false)) return FA_B200_ERR_HEADDIM;
+  if (p->dtype != FA_B200_F16 && p->dtype != FA_B200_BF16) return FA_B200_ERR_DTYPE;
+  if (p->b < 0 || p->b > 65535 || p->h <= 0 || p->h_k <= 0 || p->h_k > 65535 || p->seqlen_q <= 0 || p->num_blocks < 0 ||
+      p->max_blocks_per_seq < 0 || p->num_pages <= 0 || p->sink_pages < 0 || p->recent_pages < 0)
+    return FA_B200_ERR_SHAPE;
+  if (p->h % p->h_k != 0 || static_cast<int64_t>(p->h / p->h_k) * p->seqlen_q > 16) return FA_B200_ERR_HEADS;
+  if (!budget_page_ok(p->page_size)) return FA_B200_ERR_PAGE;
+  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > (1ll << 30)) return FA_B200_ERR_TOO_LARGE;
+  // the pages that are always taken have to fit: sq consecutive tokens lie in at most (sq - 2) / page + 2 pages (sq > 1)
+  const int open = p->seqlen_q > 1 ? (p->seqlen_q - 2) / p->page_size + 2 : 1;
+  const int64_t always = static_cast<int64_t>(p->sink_pages) + (p->recent_pages > open ? p->recent_pages : open);
+  return always <= p->num_pages ? FA_B200_OK : FA_B200_ERR_SHAPE;
+}
+
+size_t fa_b200_page_select_workspace_bytes(const fa_b200_page_select_params* p) {
+  return page_select_status(p) == FA_B200_OK ? page_select_workspace_bytes(p->b, p->h_k, p->max_blocks_per_seq) : 0;
+}
+
+int fa_b200_page_select(const fa_b200_page_select_params* p, void* stream) {
+  const int st = page_select_status(p);
+  if (st != FA_B200_OK) return st;
+  if (p->b == 0) return FA_B200_OK;
+  if (!p->q || !p->cache_seqlens || !p->page_table || !p->page_index || !p->seqlens_out) return FA_B200_ERR_NULL;
+  if (p->max_blocks_per_seq > 0 && (!p->page_bounds || !p->block_table)) return FA_B200_ERR_NULL;
+  if (!aligned16(p->q) || !aligned16(p->page_bounds)) return FA_B200_ERR_ALIGN;
+  if (!stride_ok(p->q_batch_stride, 2) || !stride_ok(p->q_row_stride, 2) || !stride_ok(p->q_head_stride, 2)) return FA_B200_ERR_STRIDE;
+  const size_t need = page_select_workspace_bytes(p->b, p->h_k, p->max_blocks_per_seq);
+  if (need > 0 && (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace))) return FA_B200_ERR_WORKSPACE;
+  PageSelectParams k{};
+  k.status = status_ptr();
+  if (!k.status) return cuda_fail("status word", cudaGetLastError());
+  k.q = p->q;
+  k.q_b = p->q_batch_stride; k.q_r = p->q_row_stride; k.q_h = p->q_head_stride;
+  k.bounds = p->page_bounds;
+  k.block_table = p->block_table;
+  k.bt_stride = p->block_table_batch_stride;
+  k.seqlens = p->cache_seqlens;
+  k.page_table = p->page_table; k.page_index = p->page_index; k.seqlens_out = p->seqlens_out;
+  k.b = p->b; k.sq = p->seqlen_q; k.h = p->h; k.h_k = p->h_k; k.group = p->h / p->h_k; k.d = p->d;
+  k.page_size = p->page_size; k.num_blocks = p->num_blocks; k.max_blocks = p->max_blocks_per_seq;
+  k.num_pages = p->num_pages; k.sink_pages = p->sink_pages; k.recent_pages = p->recent_pages;
+  k.workspace = p->workspace;
+  const cudaError_t e = launch_page_select(p->dtype, k, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("page select launch", e);
+  g_launches += p->max_blocks_per_seq > p->num_pages ? 2 : 1;
+  return FA_B200_OK;
+}
+
+// Shares of the query tiles per key tile: enough CTAs for about four rounds of the 296 CTA slots (148 SMs x 2; under a
+// causal mask a CTA's work runs from all query tiles to one), as long as a share keeps at least eight tiles.
+static int token_weights_chunks(const fa_b200_token_weights_params* p, int max_len) {
+  const int tt = 128 / (p->h / p->h_k);
+  const int64_t ctas = static_cast<int64_t>((max_len + 127) / 128) * p->h_k * p->b;
+  const int64_t tiles = (p->max_seqlen_q + tt - 1) / tt;
+  int64_t c = ctas > 0 ? (1184 + ctas - 1) / ctas : 1;
+  if (c > tiles / 8) c = tiles / 8;
+  if (c > 16) c = 16;
+  return c < 1 ? 1 : static_cast<int>(c);
+}
+static int token_weights_status(const fa_b200_token_weights_params* p) {
+  if (!p) return FA_B200_ERR_NULL;
+  if (p->struct_size != sizeof(fa_b200_token_weights_params)) return FA_B200_ERR_ABI;
+  if (!head_dim_ok(p->d, false)) return FA_B200_ERR_HEADDIM;
+  if (p->dtype != FA_B200_F16 && p->dtype != FA_B200_BF16) return FA_B200_ERR_DTYPE;
+  if (p->b < 0 || p->b > 65535 || p->h <= 0 || p->h_k <= 0 || p->h_k > 65535 || p->max_seqlen_q < 0 || p->total_q < 0 ||
+      p->total_q > 0x7fffffff || p->num_blocks < 0 || p->max_blocks_per_seq < 0 || p->weights_capacity < 0)
+    return FA_B200_ERR_SHAPE;
+  if (p->h % p->h_k != 0 || p->h / p->h_k > 128) return FA_B200_ERR_HEADS;
+  if (!budget_page_ok(p->page_size)) return FA_B200_ERR_PAGE;
+  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > 65535ll * 128) return FA_B200_ERR_TOO_LARGE;
+  return FA_B200_OK;
+}
+static int token_weights_max_len(const fa_b200_token_weights_params* p) { return p->max_blocks_per_seq * p->page_size; }
+
+size_t fa_b200_token_weights_workspace_bytes(const fa_b200_token_weights_params* p) {
+  if (token_weights_status(p) != FA_B200_OK) return 0;
+  const int max_len = token_weights_max_len(p), chunks = token_weights_chunks(p, max_len);
+  return chunks > 1 ? static_cast<size_t>(chunks) * p->b * p->h_k * max_len * sizeof(float) : 0;
+}
+
+int fa_b200_token_weights(const fa_b200_token_weights_params* p, void* stream) {
+  const int st = token_weights_status(p);
+  if (st != FA_B200_OK) return st;
+  const int max_len = token_weights_max_len(p);
+  if (p->b == 0 || max_len == 0) return FA_B200_OK;
+  if (!p->cu_seqlens_q || !p->cache_seqlens || !p->block_table || !p->k_cache || !p->weights_out) return FA_B200_ERR_NULL;
+  if (p->total_q > 0 && (!p->q || !p->softmax_lse)) return FA_B200_ERR_NULL;
+  if (!aligned16(p->q) || !aligned16(p->k_cache)) return FA_B200_ERR_ALIGN;
+  if (!stride_ok(p->q_row_stride, 2) || !stride_ok(p->q_head_stride, 2) || !stride_ok(p->k_block_stride, 2) ||
+      !stride_ok(p->k_row_stride, 2) || !stride_ok(p->k_head_stride, 2) || p->weights_in_batch_stride < 0 ||
+      p->weights_in_head_stride < 0 || p->weights_out_batch_stride < 0 || p->weights_out_head_stride < 0)
+    return FA_B200_ERR_STRIDE;
+  const size_t need = fa_b200_token_weights_workspace_bytes(p);
+  if (need > 0 && (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace))) return FA_B200_ERR_WORKSPACE;
+  TokenWeightsParams k{};
+  k.group = p->h / p->h_k;
+  k.tile_tokens = 128 / k.group;
+  k.box_rows = p->page_size >= 128 && p->page_size % 128 == 0 ? 128 : (p->page_size >= 64 ? 64 : p->page_size);
+  CUtensorMap tq, tk;
+  int s = make_tmap(&tq, p->q, p->dtype, p->h, p->total_q, 1, p->q_head_stride, p->q_row_stride,
+                    p->q_row_stride * (p->total_q > 0 ? p->total_q : 1), k.tile_tokens, p->d, k.group);
+  if (s != FA_B200_OK) return s;
+  s = make_tmap(&tk, p->k_cache, p->dtype, p->h_k, p->page_size, p->num_blocks, p->k_head_stride, p->k_row_stride, p->k_block_stride,
+                k.box_rows, p->d);
+  if (s != FA_B200_OK) return s;
+  k.status = status_ptr();
+  if (!k.status) return cuda_fail("status word", cudaGetLastError());
+  k.lse = p->softmax_lse;
+  k.lse_h = p->lse_head_stride;
+  k.cu_q = p->cu_seqlens_q;
+  k.block_table = p->block_table;
+  k.bt_stride = p->block_table_batch_stride;
+  k.seqlens = p->cache_seqlens;
+  k.w_in = p->weights_in; k.w_out = p->weights_out;
+  k.win_b = p->weights_in_batch_stride; k.win_h = p->weights_in_head_stride;
+  k.wout_b = p->weights_out_batch_stride; k.wout_h = p->weights_out_head_stride;
+  k.capacity = p->weights_capacity;
+  k.decay = p->decay;
+  k.b = p->b; k.h = p->h; k.h_k = p->h_k; k.d = p->d;
+  k.page_size = p->page_size;
+  k.max_len = max_len;
+  k.causal = p->is_causal ? 1 : 0;
+  k.scale_log2 = p->softmax_scale * kLog2e;
+  k.total_q = p->total_q;
+  k.num_chunks = token_weights_chunks(p, max_len);
+  k.partial = static_cast<float*>(p->workspace);
+  k.partial_stride = max_len;
+  const cudaError_t e = launch_token_weights(p->dtype, tq, tk, k, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("token weights launch", e);
+  g_launches += k.num_chunks > 1 ? 2 : 1;
+  return FA_B200_OK;
+}
+
+int fa_b200_kv_evict(const fa_b200_kv_evict_params* p, void* stream) {
+  if (!p) return FA_B200_ERR_NULL;
+  if (p->struct_size != sizeof(fa_b200_kv_evict_params)) return FA_B200_ERR_ABI;
+  if (!head_dim_ok(p->d, false)) return FA_B200_ERR_HEADDIM;
+  const bool fp8 = p->dtype == FA_B200_E4M3 || p->dtype == FA_B200_E5M2;
+  if (!fp8 && p->dtype != FA_B200_F16 && p->dtype != FA_B200_BF16) return FA_B200_ERR_DTYPE;
+  if (p->b < 0 || p->b > 65535 || p->h_k <= 0 || p->h_k > 32767 || p->num_blocks < 0 || p->max_blocks_per_seq < 0 ||
+      p->new_max_blocks_per_seq < 0 || p->weights_capacity < 0 || p->budget <= 0 || p->sink_tokens < 0 || p->recent_tokens < 0 ||
+      static_cast<int64_t>(p->sink_tokens) + p->recent_tokens > p->budget)
+    return FA_B200_ERR_SHAPE;
+  if (!budget_page_ok(p->page_size)) return FA_B200_ERR_PAGE;
+  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > (1ll << 30) || p->budget > (1 << 30)) return FA_B200_ERR_TOO_LARGE;
+  if (p->b == 0) return FA_B200_OK;
+  if (!p->k_cache || !p->v_cache || !p->block_table || !p->cache_seqlens || !p->weights_in || !p->weights_out || !p->kept_index ||
+      !p->seqlens_out)
+    return FA_B200_ERR_NULL;
+  const int es = fp8 ? 1 : 2;
+  if (!aligned16(p->k_cache) || !aligned16(p->v_cache)) return FA_B200_ERR_ALIGN;
+  if (!stride_ok(p->k_block_stride, es) || !stride_ok(p->k_row_stride, es) || !stride_ok(p->k_head_stride, es) ||
+      !stride_ok(p->v_block_stride, es) || !stride_ok(p->v_row_stride, es) || !stride_ok(p->v_head_stride, es) ||
+      p->weights_in_batch_stride < 0 || p->weights_in_head_stride < 0 || p->weights_out_batch_stride < 0 || p->weights_out_head_stride < 0)
+    return FA_B200_ERR_STRIDE;
+  KvEvictParams k{};
+  k.status = status_ptr();
+  if (!k.status) return cuda_fail("status word", cudaGetLastError());
+  k.k_cache = p->k_cache; k.v_cache = p->v_cache;
+  k.k_blk = p->k_block_stride * es; k.k_row = p->k_row_stride * es; k.k_h = p->k_head_stride * es;
+  k.v_blk = p->v_block_stride * es; k.v_row = p->v_row_stride * es; k.v_h = p->v_head_stride * es;
+  k.block_table = p->block_table; k.bt_stride = p->block_table_batch_stride;
+  k.new_block_table = p->new_block_table; k.nbt_stride = p->new_block_table_batch_stride;
+  k.seqlens = p->cache_seqlens;
+  k.w_in = p->weights_in; k.w_out = p->weights_out;
+  k.win_b = p->weights_in_batch_stride; k.win_h = p->weights_in_head_stride;
+  k.wout_b = p->weights_out_batch_stride; k.wout_h = p->weights_out_head_stride;
+  k.capacity = p->weights_capacity;
+  k.kept = p->kept_index; k.seqlens_out = p->seqlens_out;
+  k.b = p->b; k.h_k = p->h_k; k.row_bytes = p->d * es;
+  k.page_size = p->page_size; k.num_blocks = p->num_blocks; k.max_blocks = p->max_blocks_per_seq;
+  k.new_max_blocks = p->new_max_blocks_per_seq;
+  k.budget = p->budget; k.sink = p->sink_tokens; k.recent = p->recent_tokens;
+  const cudaError_t e = launch_kv_evict(k, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("kv evict launch", e);
+  g_launches += 2;
+  return FA_B200_OK;
+}
 
 int fa_b200_block_pool(const void* x, int32_t dtype, int64_t batch_stride, int64_t head_stride, int64_t row_stride,
                        int32_t b, int32_t h, int32_t n, int32_t d, int32_t block_rows, const float* sim_threshold,

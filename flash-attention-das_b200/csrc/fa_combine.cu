@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const Combi
   const int bi = row / (p.h * sq), hi = (row / sq) % p.h, ti = row % sq;
   int nparts = p.num_parts;
   if (p.parts_per_row) nparts = min(nparts, p.parts_per_row[bi]);
-  else if (p.seqlens) nparts = min(nparts, (p.seqlens[bi] + p.partition_tokens - 1) / p.partition_tokens);
+  else if (p.seqlens) nparts = min(nparts, (p.seqlens[bi * p.len_b + (hi / p.group) * p.len_h] + p.partition_tokens - 1) / p.partition_tokens);
 
   float mx = -INFINITY;
   for (int i = threadIdx.x; i < nparts; i += kCombineWarps * 32) {

@@ -24,7 +24,9 @@ namespace {
 // cache is e4m3, the queries (and the output) are 16-bit.  K is then converted to f16 in registers on its way into the
 // Q K^T product (f16 MMA; bf16 queries are converted to f16 once per CTA), V as in the all-e4m3 mode.
 // E5 (mixed mode only): the cache bytes are e5m2.
-template <int DT, int STAGES, bool VT, int QT = DT, int HD = 128, bool E5 = false>
+// SC: the scaled scores are also written to p.scores, for the weight that every key receives (fa_token_weights.cu); a
+// template parameter, so that the tile loop without it stays as it is.
+template <int DT, int STAGES, bool VT, int QT = DT, int HD = 128, bool E5 = false, bool SC = false>
 __global__ void __launch_bounds__(kDecodeThreads, HD > 128 ? 1 : 2)
 decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                     const DecodeKernelParams p) {
@@ -66,7 +68,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   griddep_wait();
   griddep_launch_dependents();
   // A length beyond what the block table covers would walk past the table row: cut it and report it.
-  int len = p.seqlens[b];
+  int len = p.seqlens[b * p.len_b + hk * p.len_h];
   if (len > p.max_len) {
     len = p.max_len;
     if (threadIdx.x == 0 && part == 0) atomicOr(p.status, 0x10000);
@@ -85,7 +87,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     // This partition's slice of the block table -> shared memory
     const int first_page = tok_begin / p.page_size;
     const int n_pages = (tok_end > tok_begin) ? (tok_end - 1) / p.page_size - first_page + 1 : 0;
-    load_page_ids(p.block_table + static_cast<int64_t>(b) * p.bt_stride + first_page, n_pages, sm_pages, lane);
+    load_page_ids(p.block_table + static_cast<int64_t>(b) * p.bt_stride + hk * p.bt_head_stride + first_page, n_pages, sm_pages, lane);
   }
   __syncthreads();
 
@@ -123,12 +125,13 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     if (p.q_descale) scale_log2 *= p.q_descale[b * p.qds_b + hk * p.qds_h];
     if (p.k_descale) scale_log2 *= p.k_descale[b * p.kds_b + hk * p.kds_h];
 
+    const ScoreOut so = SC ? score_out(p, b, hk, lane) : ScoreOut{};
     for (int t = 0; t < n_tiles; ++t) {
       const int s = t % STAGES;
       const uint32_t ph = (t / STAGES) & 1;
       if (!mbar_wait(smem_u32(&full_bar[s]), ph, wctx)) break;
-      consume_tile<DT, VT, QT, HD, E5>(smem_u32(stages + s * kStageBytes), tok_begin + t * T::kTile, tok_end, cw, lane, qf, lim,
-                                       scale_log2, m_run, l_run, o);
+      consume_tile<DT, VT, QT, HD, E5, SC>(smem_u32(stages + s * kStageBytes), tok_begin + t * T::kTile, tok_end, cw, lane, qf, lim,
+                                           scale_log2, m_run, l_run, o, so);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
     }
@@ -254,12 +257,14 @@ static size_t decode_smem_bytes(int stages, int stage_bytes) {
 }
 int decode_max_pages_per_partition() { return kMaxPagesPerPartition; }
 
-template <int DT, bool VT, int QT = DT, int HD = 128, bool E5 = false>
+template <int DT, bool VT, int QT = DT, int HD = 128, bool E5 = false, bool SC = false>
 static cudaError_t launch_decode_dt(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeKernelParams& p,
                                     cudaStream_t stream) {
+  if constexpr (!SC && !VT)
+    if (p.scores) return launch_decode_dt<DT, VT, QT, HD, E5, true>(tk, tv, p, stream);
   // about 96 KB of tiles in flight per CTA at two CTAs per SM; one CTA per SM above d = 128
   constexpr int STAGES = HD == 64 ? 6 : (HD == 192 ? 4 : 3);
-  auto kern = decode_paged_kernel<DT, STAGES, VT, QT, HD, E5>;
+  auto kern = decode_paged_kernel<DT, STAGES, VT, QT, HD, E5, SC>;
   const size_t smem = decode_smem_bytes(STAGES, DecodeTraits<DT, HD>::kStageBytes);
   static bool attr_done[64] = {};
   int dev = 0;

@@ -167,13 +167,22 @@ __device__ __forceinline__ RowLimits row_limits(const DecodeKernelParams& p, int
   return r;
 }
 
+// Where a thread's scores of the rows g and g + 8 of the query tile go: [b][h_k][row][score_stride], tokens contiguous;
+// nullptr: a row past sq * group.
+struct ScoreOut { float* r0; float* r1; };
+__device__ __forceinline__ ScoreOut score_out(const DecodeKernelParams& p, int b, int hk, int lane) {
+  const int g = lane >> 2, rows = p.sq * p.group;
+  float* base = p.scores + (static_cast<int64_t>(b) * p.h_k + hk) * rows * p.score_stride;
+  return ScoreOut{g < rows ? base + g * p.score_stride : nullptr, g + 8 < rows ? base + (g + 8) * p.score_stride : nullptr};
+}
+
 // One consumer warp's share of one landed K/V tile (tokens tok0 .. tok0 + kTile, those below tok_end are real): the
 // warp owns kRowsPerWarp token rows of the tile and all 16 query rows; S = Q K^T with register-level MMAs, online
 // softmax in the base-2 domain, O += P V.
-template <int DT, bool VT, int QT, int HD, bool E5, int NQ>
+template <int DT, bool VT, int QT, int HD, bool E5, bool SC, int NQ>
 __device__ __forceinline__ void consume_tile(uint32_t kbase, int tok0, int tok_end, int cw, int lane, const uint32_t (&qf)[NQ][4],
                                              const RowLimits& lim, float scale_log2, float (&m_run)[2], float (&l_run)[2],
-                                             float (&o)[DecodeTraits<DT, HD>::kNT][4]) {
+                                             float (&o)[DecodeTraits<DT, HD>::kNT][4], const ScoreOut so) {
   using T = DecodeTraits<DT, HD>;
   constexpr bool kMixed = (QT != DT);
   const int g = lane >> 2, qd = lane & 3;
@@ -225,6 +234,13 @@ __device__ __forceinline__ void consume_tile(uint32_t kbase, int tok0, int tok_e
     }
     // ---- online softmax (base-2 domain), rows g and g+8
     const int tokb = tok0 + r0 + 2 * qd;
+    if constexpr (SC) {   // every token of the sub-block, also those past the end: the rows are padded to whole tiles
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        if (so.r0) *reinterpret_cast<float2*>(so.r0 + tokb + nt * 8) = make_float2(sc[nt][0] * scale_log2, sc[nt][1] * scale_log2);
+        if (so.r1) *reinterpret_cast<float2*>(so.r1 + tokb + nt * 8) = make_float2(sc[nt][2] * scale_log2, sc[nt][3] * scale_log2);
+      }
+    }
     float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {

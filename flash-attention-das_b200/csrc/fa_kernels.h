@@ -14,6 +14,8 @@ struct DecodeKernelParams {
   void* out;
   float* lse_out;
   const int32_t* block_table;
+  int64_t bt_head_stride;   // page lists per kv head: block_table is (b, h_k, n); 0: one list per sequence
+  int32_t len_b, len_h;     // length of (sequence, kv head): seqlens[b * len_b + hk * len_h]
   const int32_t* seqlens;
   const float* q_descale;
   const float* k_descale;
@@ -48,6 +50,8 @@ struct DecodeKernelParams {
   int* tickets;
   int32_t merge_lse_empty_is_neg;   // merged rows without keys: LSE -inf (partial convention) instead of +inf
   int32_t merge_sink;               // the merge adds the sink (s_aux) to the row sums
+  float* scores;                    // [b][h_k][sq * group][score_stride] fp32, log2 units, or nullptr: see launch_token_weights_finish
+  int64_t score_stride;
   int32_t dependent_launch;         // launch with programmatic stream serialisation (the kernel waits by itself)
   int32_t test_withhold;            // FA_B200_TEST_HOOKS builds only: CTA (0, 0, 0) announces its first tile and never loads it
 };
@@ -63,7 +67,8 @@ struct CombineKernelParams {
   int64_t o_part_stride, lse_part_stride;
   void* out;
   float* lse;
-  const int32_t* seqlens;    // optional: row r uses ceil(seqlens[r / h] / partition_tokens) parts
+  const int32_t* seqlens;    // optional: row r uses ceil(length of its (sequence, kv head) / partition_tokens) parts
+  int32_t len_b, len_h, group;   // that length: seqlens[b * len_b + (head / group) * len_h]
   const int32_t* parts_per_row;  // optional explicit count per batch entry
   int64_t out_row_stride;    // rows are (b, h, tok): element offset = b * out_batch_stride + h * out_row_stride + tok * out_tok_stride
   int64_t out_batch_stride;
@@ -216,6 +221,101 @@ struct BlockSelectParams {
   int32_t is_causal, attention_sink;
   uint8_t* block_map;        // (b, h, nq, nk)
 };
+// Decode with a bounded KV cache (fa_page_select.cu, fa_kv_evict.cu, fa_token_weights.cu).
+constexpr int kRangeBit = 0x10000;   // bit of the device status word: a position or page id out of range was skipped
+struct PageBoundsParams {
+  int* status;
+  const void* k_cache;
+  int64_t k_blk, k_row, k_h;
+  void* bounds;              // (num_blocks, h_k, 2, d)
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* seqlens;
+  int32_t b, h_k, d, page_size, num_blocks, max_blocks;
+  int32_t new_tokens, slots; // slots: pages looked at per sequence
+};
+cudaError_t launch_page_bounds(int dtype, int bounds_dtype, const PageBoundsParams& p, cudaStream_t stream);
+
+struct PageSelectParams {
+  int* status;
+  const void* q;
+  int64_t q_b, q_r, q_h;
+  const void* bounds;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* seqlens;
+  int32_t* page_table;
+  int32_t* page_index;
+  int32_t* seqlens_out;
+  int32_t b, sq, h, h_k, group, d, page_size, num_blocks, max_blocks;
+  int32_t num_pages, sink_pages, recent_pages;
+  void* workspace;
+};
+size_t page_select_workspace_bytes(int b, int h_k, int max_blocks);
+cudaError_t launch_page_select(int dtype, const PageSelectParams& p, cudaStream_t stream);
+
+// weights_out = decay * weights_in + sum over the rows of 2^(score - lse): second pass of a decode that wrote its
+// scores (DecodeKernelParams::scores) and its merged lse.
+struct WeightsFinishParams {
+  const float* scores;
+  int64_t score_stride;
+  const float* lse;          // (b, h, sq), natural log
+  const int32_t* seqlens;
+  const float* w_in;
+  float* w_out;
+  int64_t win_b, win_h, wout_b, wout_h;
+  int32_t b, h, h_k, group, sq, max_len, capacity;
+  int32_t causal, window_left;
+  float decay;
+  int32_t dependent_launch;
+};
+cudaError_t launch_weights_finish(const WeightsFinishParams& p, cudaStream_t stream);
+
+struct KvEvictParams {
+  int* status;
+  void* k_cache;
+  void* v_cache;
+  int64_t k_blk, k_row, k_h, v_blk, v_row, v_h;   // strides in BYTES
+  const int32_t* block_table;
+  const int32_t* new_block_table;                  // nullptr: in place
+  int64_t bt_stride, nbt_stride;
+  const int32_t* seqlens;
+  const float* w_in;
+  float* w_out;
+  int64_t win_b, win_h, wout_b, wout_h;
+  int32_t capacity;
+  int32_t* kept;
+  int32_t* seqlens_out;
+  int32_t b, h_k, row_bytes, page_size, num_blocks, max_blocks, new_max_blocks;
+  int32_t budget, sink, recent;
+};
+cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t stream);
+
+struct TokenWeightsParams {
+  int* status;
+  const float* lse;
+  int64_t lse_h;
+  const int32_t* cu_q;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* seqlens;
+  const float* w_in;
+  float* w_out;
+  int64_t win_b, win_h, wout_b, wout_h;
+  int32_t capacity;
+  float decay;
+  int32_t b, h, h_k, group, d, page_size, box_rows, max_len;
+  int32_t causal;
+  float scale_log2;
+  int32_t tile_tokens;       // query tokens in a tile: its rows are tile_tokens x group
+  int64_t total_q;
+  int32_t num_chunks;        // query tiles are split into num_chunks interleaved shares per key tile
+  float* partial;            // [num_chunks][b][h_k][partial_stride], when num_chunks > 1
+  int64_t partial_stride;
+};
+cudaError_t launch_token_weights(int dtype, const CUtensorMap& tmap_q, const CUtensorMap& tmap_k, const TokenWeightsParams& p,
+                                 cudaStream_t stream);
+
 int block_select_max_key_blocks();
 cudaError_t launch_block_pool(const BlockPoolParams& p, cudaStream_t stream);
 cudaError_t launch_block_select(const BlockSelectParams& p, cudaStream_t stream);

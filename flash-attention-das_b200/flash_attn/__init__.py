@@ -15,5 +15,13 @@ from .flash_attn_interface import (  # noqa: F401
     vllm_flash_attn_varlen_func,
     vllm_flash_attn_with_kvcache,
 )
+from .kvcache_budget import (  # noqa: F401
+    attn_token_weights,
+    flash_attn_with_kvcache_weights,
+    kvcache_evict,
+    kvcache_page_bounds,
+    kvcache_select_pages,
+    sparse_attn_with_kvcache,
+)
 from . import torch_ops  # noqa: F401,E402  (registers flash_attn::_flash_attn_forward, flash_attn2_c_op::varlen_fwd / fwd_kvcache)
 from . import split_kv_parallel  # noqa: F401,E402  (multi-GPU helpers: sharding, partial all-gather + combine)

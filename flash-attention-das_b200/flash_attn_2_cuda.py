@@ -154,6 +154,81 @@ class KvAppendParams(_SizedStruct):
     ]
 
 
+class PageBoundsParams(_SizedStruct):
+    """struct fa_b200_page_bounds_params (include/fa_b200.h)."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("k_cache", _c_vp), ("k_block_stride", _c_i64), ("k_row_stride", _c_i64), ("k_head_stride", _c_i64),
+        ("page_bounds", _c_vp), ("block_table", _c_vp), ("block_table_batch_stride", _c_i64), ("cache_seqlens", _c_vp),
+        ("b", _c_i32), ("h_k", _c_i32), ("d", _c_i32),
+        ("page_size", _c_i32), ("num_blocks", _c_i32), ("max_blocks_per_seq", _c_i32),
+        ("new_tokens", _c_i32), ("dtype", _c_i32), ("bounds_dtype", _c_i32),
+    ]
+
+
+class PageSelectParams(_SizedStruct):
+    """struct fa_b200_page_select_params (include/fa_b200.h)."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("q", _c_vp), ("q_batch_stride", _c_i64), ("q_row_stride", _c_i64), ("q_head_stride", _c_i64),
+        ("page_bounds", _c_vp), ("block_table", _c_vp), ("block_table_batch_stride", _c_i64), ("cache_seqlens", _c_vp),
+        ("page_table", _c_vp), ("page_index", _c_vp), ("seqlens_out", _c_vp),
+        ("b", _c_i32), ("seqlen_q", _c_i32), ("h", _c_i32), ("h_k", _c_i32), ("d", _c_i32),
+        ("page_size", _c_i32), ("num_blocks", _c_i32), ("max_blocks_per_seq", _c_i32),
+        ("num_pages", _c_i32), ("sink_pages", _c_i32), ("recent_pages", _c_i32), ("dtype", _c_i32),
+        ("workspace", _c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class DecodeBudgetParams(_SizedStruct):
+    """struct fa_b200_decode_budget_params (include/fa_b200.h)."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("per_kv_head", _c_i32), ("block_table_head_stride", _c_i64),
+        ("weights_in", _c_vp), ("weights_out", _c_vp),
+        ("weights_in_batch_stride", _c_i64), ("weights_in_head_stride", _c_i64),
+        ("weights_out_batch_stride", _c_i64), ("weights_out_head_stride", _c_i64),
+        ("weights_capacity", _c_i32), ("decay", _c_f32),
+    ]
+
+
+class TokenWeightsParams(_SizedStruct):
+    """struct fa_b200_token_weights_params (include/fa_b200.h)."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("q", _c_vp), ("q_row_stride", _c_i64), ("q_head_stride", _c_i64),
+        ("softmax_lse", _c_vp), ("lse_head_stride", _c_i64), ("cu_seqlens_q", _c_vp),
+        ("k_cache", _c_vp), ("k_block_stride", _c_i64), ("k_row_stride", _c_i64), ("k_head_stride", _c_i64),
+        ("block_table", _c_vp), ("block_table_batch_stride", _c_i64), ("cache_seqlens", _c_vp),
+        ("weights_in", _c_vp), ("weights_out", _c_vp),
+        ("weights_in_batch_stride", _c_i64), ("weights_in_head_stride", _c_i64),
+        ("weights_out_batch_stride", _c_i64), ("weights_out_head_stride", _c_i64),
+        ("weights_capacity", _c_i32), ("decay", _c_f32), ("total_q", _c_i64),
+        ("b", _c_i32), ("max_seqlen_q", _c_i32), ("h", _c_i32), ("h_k", _c_i32), ("d", _c_i32),
+        ("page_size", _c_i32), ("num_blocks", _c_i32), ("max_blocks_per_seq", _c_i32),
+        ("softmax_scale", _c_f32), ("is_causal", _c_i32), ("dtype", _c_i32),
+        ("workspace", _c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class KvEvictParams(_SizedStruct):
+    """struct fa_b200_kv_evict_params (include/fa_b200.h)."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("k_cache", _c_vp), ("v_cache", _c_vp),
+        ("k_block_stride", _c_i64), ("k_row_stride", _c_i64), ("k_head_stride", _c_i64),
+        ("v_block_stride", _c_i64), ("v_row_stride", _c_i64), ("v_head_stride", _c_i64),
+        ("block_table", _c_vp), ("block_table_batch_stride", _c_i64),
+        ("new_block_table", _c_vp), ("new_block_table_batch_stride", _c_i64), ("cache_seqlens", _c_vp),
+        ("weights_in", _c_vp), ("weights_out", _c_vp),
+        ("weights_in_batch_stride", _c_i64), ("weights_in_head_stride", _c_i64),
+        ("weights_out_batch_stride", _c_i64), ("weights_out_head_stride", _c_i64),
+        ("weights_capacity", _c_i32), ("kept_index", _c_vp), ("seqlens_out", _c_vp),
+        ("b", _c_i32), ("h_k", _c_i32), ("d", _c_i32),
+        ("page_size", _c_i32), ("num_blocks", _c_i32), ("max_blocks_per_seq", _c_i32), ("new_max_blocks_per_seq", _c_i32),
+        ("budget", _c_i32), ("sink_tokens", _c_i32), ("recent_tokens", _c_i32), ("dtype", _c_i32),
+    ]
+
+
 _lib.fa_b200_fwd.argtypes = [ctypes.POINTER(FwdParams), _c_vp]
 _lib.fa_b200_fwd.restype = ctypes.c_int
 _lib.fa_b200_fwd_sparse.argtypes = [ctypes.POINTER(FwdParams), _c_vp]
@@ -207,6 +282,22 @@ _lib.fa_b200_exchange_combine.argtypes = [ctypes.POINTER(ExchangeParams), _c_vp]
 _lib.fa_b200_exchange_combine.restype = ctypes.c_int
 _lib.fa_b200_read_stream.argtypes = [_c_vp, _c_i64, _c_vp, _c_vp]
 _lib.fa_b200_read_stream.restype = ctypes.c_int
+_lib.fa_b200_page_bounds.argtypes = [ctypes.POINTER(PageBoundsParams), _c_vp]
+_lib.fa_b200_page_bounds.restype = ctypes.c_int
+_lib.fa_b200_page_select.argtypes = [ctypes.POINTER(PageSelectParams), _c_vp]
+_lib.fa_b200_page_select.restype = ctypes.c_int
+_lib.fa_b200_page_select_workspace_bytes.argtypes = [ctypes.POINTER(PageSelectParams)]
+_lib.fa_b200_page_select_workspace_bytes.restype = ctypes.c_size_t
+_lib.fa_b200_decode_budget.argtypes = [ctypes.POINTER(DecodeParams), ctypes.POINTER(DecodeBudgetParams), _c_vp]
+_lib.fa_b200_decode_budget.restype = ctypes.c_int
+_lib.fa_b200_decode_budget_workspace_bytes.argtypes = [ctypes.POINTER(DecodeParams), ctypes.POINTER(DecodeBudgetParams)]
+_lib.fa_b200_decode_budget_workspace_bytes.restype = ctypes.c_size_t
+_lib.fa_b200_token_weights.argtypes = [ctypes.POINTER(TokenWeightsParams), _c_vp]
+_lib.fa_b200_token_weights.restype = ctypes.c_int
+_lib.fa_b200_token_weights_workspace_bytes.argtypes = [ctypes.POINTER(TokenWeightsParams)]
+_lib.fa_b200_token_weights_workspace_bytes.restype = ctypes.c_size_t
+_lib.fa_b200_kv_evict.argtypes = [ctypes.POINTER(KvEvictParams), _c_vp]
+_lib.fa_b200_kv_evict.restype = ctypes.c_int
 _lib.fa_b200_set_print_param.argtypes = [ctypes.c_int]
 _lib.fa_b200_set_print_param.restype = None
 _lib.fa_b200_last_launch_info.restype = ctypes.c_char_p
@@ -1193,6 +1284,236 @@ def block_select(pooled_q, pooled_k, sim_q, sim_k, block_q, block_k, scale, cdf_
 
 # ------------------------------------------------------------------------------------------------
 # torch.library ops the reference's compiled extension defines on import
+# ------------------------------------------------------------------------------------------------
+# decode with a bounded KV cache
+# ------------------------------------------------------------------------------------------------
+_DT_CACHE = {**_DT, torch.float8_e5m2: 4}
+
+
+def _check_cache(k_cache, block_table, cache_seqlens, what, v_cache=None):
+    """A paged pool (num_blocks, page, h_k, d) with d contiguous, its block table (b, n) and the sequences' lengths (b)."""
+    _require(k_cache.is_cuda and k_cache.dim() == 4 and k_cache.stride(3) == 1,
+             f"{what}: k_cache must be a CUDA tensor (num_blocks, page_size, nheads_k, d) with contiguous last dimension")
+    _require(k_cache.dtype in _DT_CACHE, f"{what}: the cache must be fp16, bf16, fp8 e4m3 or fp8 e5m2")
+    if v_cache is not None:
+        _require(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype and v_cache.device == k_cache.device and
+                 v_cache.stride(3) == 1, f"{what}: v_cache must be like k_cache, with contiguous last dimension")
+    _check_tables(block_table, cache_seqlens, k_cache.device, what)
+
+
+def _check_tables(block_table, cache_seqlens, device, what):
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.device == device and
+             (block_table.stride(1) == 1 or block_table.shape[1] <= 1),
+             f"{what}: block_table must be an int32 tensor (batch, max_num_blocks_per_seq) on the cache's device with "
+             "contiguous last dimension")
+    _require(cache_seqlens.dtype == torch.int32 and cache_seqlens.device == device and cache_seqlens.dim() == 1 and
+             cache_seqlens.shape[0] == block_table.shape[0] and cache_seqlens.is_contiguous(),
+             f"{what}: cache_seqlens must be a contiguous int32 tensor (batch,) on the cache's device")
+
+
+def _set_weights(p, w_in, w_out, b, h_k, device, what):
+    """fp32 token weights (b, h_k, capacity), capacity contiguous; w_out None: in place."""
+    if w_out is None:
+        _require(w_in is not None, f"{what}: token_weights is required")
+        w_out = w_in
+    for w in (w_out,) if w_in is None or w_in is w_out else (w_in, w_out):
+        _require(w.dtype == torch.float32 and w.device == device and w.dim() == 3 and w.shape[0] == b and w.shape[1] == h_k and
+                 (w.stride(2) == 1 or w.shape[2] <= 1),
+                 f"{what}: token weights must be a float32 tensor (batch, nheads_k, capacity) on the cache's device with "
+                 "contiguous last dimension")
+    os_ = w_out.stride()
+    p.weights_out, p.weights_out_batch_stride, p.weights_out_head_stride = w_out.data_ptr(), os_[0], os_[1]
+    if w_in is not None:
+        _require(w_in.shape[2] == w_out.shape[2], f"{what}: token_weights_out must have the capacity of token_weights")
+        is_ = w_in.stride()
+        p.weights_in, p.weights_in_batch_stride, p.weights_in_head_stride = w_in.data_ptr(), is_[0], is_[1]
+    p.weights_capacity = w_out.shape[2]
+    return w_out
+
+
+def page_bounds(k_cache, block_table, cache_seqlens, bounds, new_tokens=0):
+    """fa_b200_page_bounds: writes ``bounds`` (num_blocks, h_k, 2, d), fp16 / bf16."""
+    _check_cache(k_cache, block_table, cache_seqlens, "page_bounds")
+    nb, page, h_k, d = k_cache.shape
+    _require(bounds.shape == (nb, h_k, 2, d) and bounds.is_contiguous() and bounds.device == k_cache.device and
+             bounds.dtype in (torch.float16, torch.bfloat16) and
+             (k_cache.element_size() == 1 or bounds.dtype == k_cache.dtype),
+             "page_bounds: bounds must be a contiguous tensor (num_blocks, nheads_k, 2, d) of the cache's type (fp16 or bf16 "
+             "for an fp8 cache) on the cache's device")
+    p = PageBoundsParams()
+    p.k_cache, p.page_bounds = k_cache.data_ptr(), bounds.data_ptr()
+    p.k_block_stride, p.k_row_stride, p.k_head_stride, _ = k_cache.stride()
+    p.block_table, p.block_table_batch_stride = block_table.data_ptr(), block_table.stride(0)
+    p.cache_seqlens = cache_seqlens.data_ptr()
+    p.b, p.max_blocks_per_seq = block_table.shape
+    p.num_blocks, p.page_size, p.h_k, p.d = nb, page, h_k, d
+    p.new_tokens = new_tokens
+    p.dtype, p.bounds_dtype = _DT_CACHE[k_cache.dtype], _DT[bounds.dtype]
+    with _on_device(k_cache.device):
+        _check(_lib.fa_b200_page_bounds(ctypes.byref(p), _stream(k_cache)), "page_bounds")
+    return bounds
+
+
+def page_select(q, bounds, block_table, cache_seqlens, page_size, num_pages, sink_pages=1, recent_pages=1):
+    """fa_b200_page_select: (page_table, seqlens, page_index)."""
+    _require(q.is_cuda and q.dim() == 4 and q.stride(3) == 1 and q.dtype in (torch.float16, torch.bfloat16),
+             "page_select: q must be an fp16 / bf16 CUDA tensor (batch, seqlen_q, nheads, d) with contiguous last dimension")
+    b, sq, h, d = q.shape
+    _require(bounds.dim() == 4 and bounds.shape[2] == 2 and bounds.shape[3] == d and bounds.is_contiguous() and
+             bounds.dtype == q.dtype and bounds.device == q.device,
+             "page_select: page_bounds must be a contiguous tensor (num_blocks, nheads_k, 2, d) of q's type on q's device")
+    _check_tables(block_table, cache_seqlens, q.device, "page_select")
+    _require(block_table.shape[0] == b, "page_select: block_table batch mismatch")
+    h_k = bounds.shape[1]
+    p = PageSelectParams()
+    p.q, p.page_bounds = q.data_ptr(), bounds.data_ptr()
+    p.q_batch_stride, p.q_row_stride, p.q_head_stride, _ = q.stride()
+    p.block_table, p.block_table_batch_stride = block_table.data_ptr(), block_table.stride(0)
+    p.cache_seqlens = cache_seqlens.data_ptr()
+    p.b, p.seqlen_q, p.h, p.h_k, p.d = b, sq, h, h_k, d
+    p.page_size, p.num_blocks, p.max_blocks_per_seq = page_size, bounds.shape[0], block_table.shape[1]
+    p.num_pages, p.sink_pages, p.recent_pages = num_pages, sink_pages, recent_pages
+    p.dtype = _DT[q.dtype]
+    _require(num_pages > 0, "page_select: num_pages must be positive")
+    # one allocation: the two tables and the lengths
+    n = b * h_k * num_pages
+    buf = torch.empty(2 * n + b * h_k, dtype=torch.int32, device=q.device)
+    p.page_table = buf.data_ptr()
+    p.page_index = p.page_table + 4 * n
+    p.seqlens_out = p.page_table + 8 * n
+    with _on_device(q.device):
+        ws = _workspace(q.device, int(_lib.fa_b200_page_select_workspace_bytes(ctypes.byref(p))))
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+        _check(_lib.fa_b200_page_select(ctypes.byref(p), _stream(q)), "page_select")
+    return buf[:n].view(b, h_k, num_pages), buf[2 * n:].view(b, h_k), buf[n:2 * n].view(b, h_k, num_pages)
+
+
+def decode_budget(q, kcache, vcache, block_table, seqlens, softmax_scale, is_causal=False, out=None, s_aux=None,
+                  window_left=-1, token_weights=None, token_weights_out=None, decay=1.0, q_descale=None, k_descale=None,
+                  v_descale=None):
+    """fa_b200_decode_budget: decode over the pages of ``block_table`` (b, n), or (b, h_k, n) with ``seqlens`` (b, h_k), and,
+    when token weights are given, the weight of every key.  Returns (out, softmax_lse, token weights or None)."""
+    v_t = _is_transposed_v(vcache)
+    _check_qkv(q, kcache, vcache, v_t, allow_fp8_kv=True)
+    _require(q.dim() == 4 and kcache.dim() == 4 and kcache.shape == vcache.shape,
+             "q must be (batch, seqlen_q, nheads, d) and k_cache / v_cache (num_blocks, page_size, nheads_k, d)")
+    b, sq, h, d = q.shape
+    h_k = kcache.shape[2]
+    dev = q.device
+    _require(kcache.device == dev and vcache.device == dev, "q and the caches must be on one device")
+    _require(h % h_k == 0, "Number of heads in key/value must divide number of heads in query")
+    _require(sq >= 1, "q must hold at least one token per sequence")
+    per_head = block_table.dim() == 3
+    _unsupported(v_t, "a transposed V pool (layout 0)")
+    _unsupported(_is_fp8_kv(q, kcache) and q_descale is not None, "an fp8 KV cache under 16-bit queries with q_descale")
+    _require(block_table.dtype == torch.int32 and block_table.device == dev and
+             (block_table.stride(-1) == 1 or block_table.shape[-1] <= 1) and
+             tuple(block_table.shape[:-1]) == ((b, h_k) if per_head else (b,)),
+             "the block table must be int32, (batch, n) or (batch, nheads_k, n), on q's device with contiguous last dimension")
+    _require(seqlens.dtype == torch.int32 and seqlens.device == dev and seqlens.is_contiguous() and
+             tuple(seqlens.shape) == ((b, h_k) if per_head else (b,)),
+             "the lengths must be a contiguous int32 tensor, (batch,) or with a table for each kv head (batch, nheads_k)")
+    odt = _out_dtype(q, out)
+    if out is not None:
+        _require(tuple(out.shape) == (b, sq, h, d) and out.stride(-1) == 1 and out.device == dev,
+                 "out must have the shape of q and a contiguous last dimension")
+    else:
+        out = torch.empty((b, sq, h, d), dtype=odt, device=dev)
+    lse = torch.empty((b, h, sq), dtype=torch.float32, device=dev)
+    e = DecodeBudgetParams()
+    w = None
+    if token_weights is not None or token_weights_out is not None:
+        w = _set_weights(e, token_weights, token_weights_out, b, h_k, dev, "token weights")
+        e.decay = decay
+    p = _decode_params(q, kcache, vcache, seqlens, block_table, softmax_scale, out, lse, q_descale, k_descale, v_descale)
+    if per_head:
+        e.per_kv_head, e.block_table_head_stride = 1, block_table.stride(1)
+        p.max_blocks_per_seq = block_table.shape[2]
+    p.is_causal = 1 if is_causal else 0
+    _set_sinks(p, s_aux, h)
+    _set_window(p, window_left, -1)
+    with _on_device(dev):
+        ws = _workspace(dev, int(_lib.fa_b200_decode_budget_workspace_bytes(ctypes.byref(p), ctypes.byref(e))))
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+            _tickets = _own_tickets(p, dev, b * h_k)
+        _check(_lib.fa_b200_decode_budget(ctypes.byref(p), ctypes.byref(e), _stream(q)), "decode_budget")
+    return out, lse, w
+
+
+def token_weights(q, k_cache, softmax_lse, cu_seqlens_q, max_seqlen_q, cache_seqlens, block_table, weights, softmax_scale,
+                  is_causal=True, decay=1.0, weights_out=None):
+    """fa_b200_token_weights: weight of every cached key under a prompt's queries, into ``weights_out`` (None: ``weights``)."""
+    _check_cache(k_cache, block_table, cache_seqlens, "token_weights")
+    dev = k_cache.device
+    _require(q.dim() == 3 and q.device == dev and q.stride(2) == 1, "token_weights: q must be (total_q, nheads, d) on the "
+             "cache's device with contiguous last dimension")
+    _unsupported(q.dtype not in (torch.float16, torch.bfloat16) or k_cache.dtype != q.dtype,
+                 "token_weights with other than fp16 or bf16 queries and a cache of their type")
+    total_q, h, d = q.shape
+    nb, page, h_k, dk = k_cache.shape
+    b = block_table.shape[0]
+    _require(dk == d and h % h_k == 0, "token_weights: q and k_cache must have the same d, and nheads_k must divide nheads")
+    _require(softmax_lse.dtype == torch.float32 and softmax_lse.device == dev and tuple(softmax_lse.shape) == (h, total_q) and
+             (softmax_lse.stride(1) == 1 or total_q <= 1), "token_weights: softmax_lse must be a float32 tensor (nheads, total_q)")
+    _require(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.device == dev and cu_seqlens_q.is_contiguous() and
+             tuple(cu_seqlens_q.shape) == (b + 1,), "token_weights: cu_seqlens_q must be a contiguous int32 tensor (batch + 1,)")
+    p = TokenWeightsParams()
+    w = _set_weights(p, weights, weights_out, b, h_k, dev, "token_weights")
+    p.q, p.softmax_lse, p.cu_seqlens_q = q.data_ptr(), softmax_lse.data_ptr(), cu_seqlens_q.data_ptr()
+    p.q_row_stride, p.q_head_stride, _ = q.stride()
+    p.lse_head_stride = softmax_lse.stride(0)
+    p.k_cache = k_cache.data_ptr()
+    p.k_block_stride, p.k_row_stride, p.k_head_stride, _ = k_cache.stride()
+    p.block_table, p.block_table_batch_stride = block_table.data_ptr(), block_table.stride(0)
+    p.cache_seqlens = cache_seqlens.data_ptr()
+    p.decay, p.total_q = decay, total_q
+    p.b, p.max_seqlen_q, p.h, p.h_k, p.d = b, max_seqlen_q, h, h_k, d
+    p.page_size, p.num_blocks, p.max_blocks_per_seq = page, nb, block_table.shape[1]
+    p.softmax_scale, p.is_causal, p.dtype = softmax_scale, 1 if is_causal else 0, _DT[q.dtype]
+    with _on_device(dev):
+        ws = _workspace(dev, int(_lib.fa_b200_token_weights_workspace_bytes(ctypes.byref(p))))
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+        _check(_lib.fa_b200_token_weights(ctypes.byref(p), _stream(k_cache)), "token_weights")
+    return w
+
+
+def kv_evict(k_cache, v_cache, block_table, cache_seqlens, weights, budget, sink_tokens, recent_tokens,
+             new_block_table=None, weights_out=None):
+    """fa_b200_kv_evict: (kept_index (b, h_k, budget), new lengths (b))."""
+    _check_cache(k_cache, block_table, cache_seqlens, "kv_evict", v_cache)
+    nb, page, h_k, d = k_cache.shape
+    b, dev = block_table.shape[0], k_cache.device
+    _require(budget > 0, "kv_evict: budget must be positive")
+    p = KvEvictParams()
+    _set_weights(p, weights, weights_out, b, h_k, dev, "kv_evict")
+    _require(weights is not None, "kv_evict: token_weights is required")
+    p.k_cache, p.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    p.k_block_stride, p.k_row_stride, p.k_head_stride, _ = k_cache.stride()
+    p.v_block_stride, p.v_row_stride, p.v_head_stride, _ = v_cache.stride()
+    p.block_table, p.block_table_batch_stride = block_table.data_ptr(), block_table.stride(0)
+    if new_block_table is not None:
+        _require(new_block_table.dtype == torch.int32 and new_block_table.dim() == 2 and new_block_table.device == dev and
+                 new_block_table.shape[0] == b and (new_block_table.stride(1) == 1 or new_block_table.shape[1] <= 1),
+                 "kv_evict: new_block_table must be like block_table")
+        p.new_block_table, p.new_block_table_batch_stride = new_block_table.data_ptr(), new_block_table.stride(0)
+        p.new_max_blocks_per_seq = new_block_table.shape[1]
+    p.cache_seqlens = cache_seqlens.data_ptr()
+    p.b, p.h_k, p.d = b, h_k, d
+    p.page_size, p.num_blocks, p.max_blocks_per_seq = page, nb, block_table.shape[1]
+    p.budget, p.sink_tokens, p.recent_tokens = budget, sink_tokens, recent_tokens
+    p.dtype = _DT_CACHE[k_cache.dtype]
+    n = b * h_k * budget
+    buf = torch.empty(n + b, dtype=torch.int32, device=dev)
+    p.kept_index = buf.data_ptr()
+    p.seqlens_out = p.kept_index + 4 * n
+    with _on_device(dev):
+        _check(_lib.fa_b200_kv_evict(ctypes.byref(p), _stream(k_cache)), "kv_evict")
+    return buf[:n].view(b, h_k, budget), buf[n:]
+
+
 # ------------------------------------------------------------------------------------------------
 # flash_attn2_c_op::varlen_fwd and ::fwd_kvcache are C++ schemas in the reference (csrc/flash_attn_cutlass/
 # flash_api.cpp:2796-2816, TORCH_LIBRARY + TORCH_LIBRARY_IMPL); its Python interface only adds fake implementations

@@ -31,7 +31,8 @@ extern "C" {
 #endif
 
 /* element types */
-enum { FA_B200_F16 = 0, FA_B200_BF16 = 1, FA_B200_E4M3 = 2, FA_B200_F32 = 3 /* s_aux only */ };
+enum { FA_B200_F16 = 0, FA_B200_BF16 = 1, FA_B200_E4M3 = 2, FA_B200_F32 = 3 /* s_aux only */,
+       FA_B200_E5M2 = 4 /* caches of fa_b200_page_bounds and fa_b200_kv_evict only */ };
 
 /* status codes (host side).  fa_b200_status_string() gives the text. */
 enum {
@@ -528,6 +529,164 @@ FA_B200_API int fa_b200_block_select(const void* pooled_q, const void* pooled_k,
                                      int32_t d, int32_t block_q, int32_t block_k, float scale,
                                      const float* cdf_threshold, const float* topk, int32_t is_causal,
                                      int32_t attention_sink, uint8_t* block_map, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Decode with a bounded KV cache: read only the pages that matter (page_bounds, page_select, decode_budget with page
+ * lists per kv head), or keep only the keys that matter (token weights from decode_budget / token_weights, kv_evict).
+ * ------------------------------------------------------------------------------------------------ */
+
+/*
+ * page_bounds[page, hk, 0, :] = smallest and [page, hk, 1, :] = largest value of every channel over the rows of a
+ * page that hold tokens (a NaN among them gives NaN), for the pages that hold the last `new_tokens` tokens of every
+ * sequence (0: all of its pages), from all of a page's rows up to the sequence's length.  Other pages' bounds are left
+ * as they are.  A page that several sequences share has to be full in all of them.  dtype: type of the cache
+ * (F16 / BF16 / E4M3 / E5M2); bounds_dtype: F16 / BF16, the cache's own type for 16-bit caches.
+ */
+typedef struct fa_b200_page_bounds_params {
+  uint32_t struct_size;                /* sizeof(struct fa_b200_page_bounds_params) */
+  const void* k_cache;                 /* (num_blocks, page_size, h_k, d), d contiguous */
+  int64_t k_block_stride, k_row_stride, k_head_stride;
+  void* page_bounds;                   /* (num_blocks, h_k, 2, d), contiguous */
+  const int32_t* block_table;          /* (b, max_blocks_per_seq), last dim contiguous */
+  int64_t block_table_batch_stride;
+  const int32_t* cache_seqlens;        /* (b) */
+  int32_t b, h_k, d;                   /* d: 64, 128, 192 or 256 */
+  int32_t page_size, num_blocks, max_blocks_per_seq;
+  int32_t new_tokens;
+  int32_t dtype, bounds_dtype;
+} fa_b200_page_bounds_params;
+
+FA_B200_API int fa_b200_page_bounds(const fa_b200_page_bounds_params* p, void* stream);
+
+/*
+ * The num_pages pages of every (sequence, kv head) that its queries may attend to most.  Score of a page: the largest,
+ * over the seqlen_q query tokens and the query heads of the kv head's group, of
+ *     sum_c max(q_c lo_c, q_c hi_c)    (no key of the page has a larger q . k)
+ * Always taken: the first sink_pages, the last recent_pages and the pages that hold the last seqlen_q tokens; then the
+ * highest scores, of equal ones the lowest page (a NaN score counts as the highest).  The choice is that of the exact
+ * scores: pages whose 32-bit scores lie too near the border are compared in 64 bits.  Outputs, in ascending order of
+ * the page's position in the sequence and padded with -1: page_index its position, page_table the physical page;
+ * seqlens_out the tokens in the chosen pages.  All of a short sequence's pages are taken.
+ */
+typedef struct fa_b200_page_select_params {
+  uint32_t struct_size;                /* sizeof(struct fa_b200_page_select_params) */
+  const void* q;                       /* (b, seqlen_q, h, d) */
+  int64_t q_batch_stride, q_row_stride, q_head_stride;
+  const void* page_bounds;             /* (num_blocks, h_k, 2, d), contiguous, element type of q */
+  const int32_t* block_table;
+  int64_t block_table_batch_stride;
+  const int32_t* cache_seqlens;
+  int32_t* page_table;                 /* out (b, h_k, num_pages) */
+  int32_t* page_index;                 /* out (b, h_k, num_pages) */
+  int32_t* seqlens_out;                /* out (b, h_k) */
+  int32_t b, seqlen_q, h, h_k, d;      /* seqlen_q * h / h_k <= 16 */
+  int32_t page_size, num_blocks, max_blocks_per_seq;
+  int32_t num_pages, sink_pages, recent_pages;
+  int32_t dtype;                       /* F16 / BF16 */
+  void* workspace;
+  size_t workspace_bytes;              /* fa_b200_page_select_workspace_bytes */
+} fa_b200_page_select_params;
+
+FA_B200_API size_t fa_b200_page_select_workspace_bytes(const fa_b200_page_select_params* p);
+FA_B200_API int fa_b200_page_select(const fa_b200_page_select_params* p, void* stream);
+
+/*
+ * fa_b200_decode_paged with two additions.
+ * per_kv_head: block_table is (b, h_k, n) with block_table_head_stride and cache_seqlens (b, h_k) contiguous: every kv
+ * head attends to its own list of pages (the outputs of fa_b200_page_select).
+ * weights_out: the weight that every key received, for the keys below the sequence's length,
+ *     weights_out[b, hk, t] = decay * weights_in[b, hk, t] + sum over query tokens and heads of the group of
+ *                             exp(score - lse)
+ * in fp32, keys contiguous, strides in elements; weights_out may be weights_in.  Keys at or past the length (or past
+ * weights_capacity) are left as they are.  weights_out needs softmax_lse and excludes per_kv_head and o_partial_out.
+ */
+typedef struct fa_b200_decode_budget_params {
+  uint32_t struct_size;                /* sizeof(struct fa_b200_decode_budget_params) */
+  int32_t per_kv_head;
+  int64_t block_table_head_stride;
+  const float* weights_in;             /* (b, h_k, weights_capacity) or null: zeros */
+  float* weights_out;                  /* (b, h_k, weights_capacity) or null: no weights */
+  int64_t weights_in_batch_stride, weights_in_head_stride;
+  int64_t weights_out_batch_stride, weights_out_head_stride;
+  int32_t weights_capacity;
+  float decay;
+} fa_b200_decode_budget_params;
+
+FA_B200_API size_t fa_b200_decode_budget_workspace_bytes(const fa_b200_decode_params* p, const fa_b200_decode_budget_params* e);
+FA_B200_API int fa_b200_decode_budget(const fa_b200_decode_params* p, const fa_b200_decode_budget_params* e, void* stream);
+
+/*
+ * The weight that every cached key received from the queries of a prompt (or of the last queries of it), from the
+ * log-sum-exp that the attention call of the prompt returned:
+ *     weights_out[b, hk, t] = decay * weights_in[b, hk, t] + sum over the sequence's queries that see key t and the
+ *                             heads of the group of exp(softmax_scale * q . k_t - lse)
+ * The queries of sequence b are rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] of q and the last positions of the
+ * sequence; with is_causal query i of n sees the keys below len - n + i + 1.  A query whose lse is +inf gives nothing.
+ */
+typedef struct fa_b200_token_weights_params {
+  uint32_t struct_size;                /* sizeof(struct fa_b200_token_weights_params) */
+  const void* q;                       /* (total_q, h, d), F16 / BF16 */
+  int64_t q_row_stride, q_head_stride;
+  const float* softmax_lse;            /* (h, total_q), rows contiguous */
+  int64_t lse_head_stride;
+  const int32_t* cu_seqlens_q;         /* (b + 1) */
+  const void* k_cache;                 /* (num_blocks, page_size, h_k, d) */
+  int64_t k_block_stride, k_row_stride, k_head_stride;
+  const int32_t* block_table;
+  int64_t block_table_batch_stride;
+  const int32_t* cache_seqlens;
+  const float* weights_in;
+  float* weights_out;
+  int64_t weights_in_batch_stride, weights_in_head_stride;
+  int64_t weights_out_batch_stride, weights_out_head_stride;
+  int32_t weights_capacity;
+  float decay;
+  int64_t total_q;
+  int32_t b, max_seqlen_q, h, h_k, d;
+  int32_t page_size, num_blocks, max_blocks_per_seq;
+  float softmax_scale;
+  int32_t is_causal;
+  int32_t dtype;
+  void* workspace;
+  size_t workspace_bytes;              /* fa_b200_token_weights_workspace_bytes */
+} fa_b200_token_weights_params;
+
+FA_B200_API size_t fa_b200_token_weights_workspace_bytes(const fa_b200_token_weights_params* p);
+FA_B200_API int fa_b200_token_weights(const fa_b200_token_weights_params* p, void* stream);
+
+/*
+ * Cuts every sequence longer than `budget` to `budget` tokens per kv head: kept are the first sink_tokens, the last
+ * recent_tokens and, of the others, those with the highest weight (equal ones: the lowest position; a NaN counts as the
+ * highest).  kept_index gets the kept positions in ascending order, padded with -1; seqlens_out min(length, budget).
+ * K, V and weights of the kept tokens move to positions 0, 1, .. in that order: in place where new_block_table is null
+ * (the pages must then belong to one sequence each), else into the pages it names, which must not be pages of
+ * block_table.  weights_out (may be weights_in) becomes zero from the new to the old length, and keeps what lies behind.
+ */
+typedef struct fa_b200_kv_evict_params {
+  uint32_t struct_size;                /* sizeof(struct fa_b200_kv_evict_params) */
+  void* k_cache;
+  void* v_cache;
+  int64_t k_block_stride, k_row_stride, k_head_stride;
+  int64_t v_block_stride, v_row_stride, v_head_stride;
+  const int32_t* block_table;
+  int64_t block_table_batch_stride;
+  const int32_t* new_block_table;      /* null: in place */
+  int64_t new_block_table_batch_stride;
+  const int32_t* cache_seqlens;
+  const float* weights_in;             /* (b, h_k, weights_capacity) */
+  float* weights_out;
+  int64_t weights_in_batch_stride, weights_in_head_stride;
+  int64_t weights_out_batch_stride, weights_out_head_stride;
+  int32_t weights_capacity;
+  int32_t* kept_index;                 /* out (b, h_k, budget) */
+  int32_t* seqlens_out;                /* out (b) */
+  int32_t b, h_k, d;
+  int32_t page_size, num_blocks, max_blocks_per_seq, new_max_blocks_per_seq;
+  int32_t budget, sink_tokens, recent_tokens;
+  int32_t dtype;
+} fa_b200_kv_evict_params;
+
+FA_B200_API int fa_b200_kv_evict(const fa_b200_kv_evict_params* p, void* stream);
 
 #ifdef __cplusplus
 }
