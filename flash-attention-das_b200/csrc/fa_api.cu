@@ -1154,7 +1154,7 @@ static int page_select_status(const fa_b200_page_select_params* p) {
     return FA_B200_ERR_SHAPE;
   if (p->h % p->h_k != 0 || static_cast<int64_t>(p->h / p->h_k) * p->seqlen_q > 16) return FA_B200_ERR_HEADS;
   if (!budget_page_ok(p->page_size)) return FA_B200_ERR_PAGE;
-  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > (1ll << 30)) return FA_B200_ERR_TOO_LARGE;
+  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > (1ll << 30) || p->max_blocks_per_seq > 65535 * 32) return FA_B200_ERR_TOO_LARGE;
   // the pages that are always taken have to fit: sq consecutive tokens lie in at most (sq - 2) / page + 2 pages (sq > 1)
   const int open = p->seqlen_q > 1 ? (p->seqlen_q - 2) / p->page_size + 2 : 1;
   const int64_t always = static_cast<int64_t>(p->sink_pages) + (p->recent_pages > open ? p->recent_pages : open);
@@ -1189,6 +1189,7 @@ int fa_b200_page_select(const fa_b200_page_select_params* p, void* stream) {
   k.page_size = p->page_size; k.num_blocks = p->num_blocks; k.max_blocks = p->max_blocks_per_seq;
   k.num_pages = p->num_pages; k.sink_pages = p->sink_pages; k.recent_pages = p->recent_pages;
   k.workspace = p->workspace;
+  k.dependent_launch = g_env.dependent_launch;
   const cudaError_t e = launch_page_select(p->dtype, k, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail("page select launch", e);
   g_launches += p->max_blocks_per_seq > p->num_pages ? 2 : 1;
@@ -1320,6 +1321,7 @@ int fa_b200_kv_evict(const fa_b200_kv_evict_params* p, void* stream) {
   k.page_size = p->page_size; k.num_blocks = p->num_blocks; k.max_blocks = p->max_blocks_per_seq;
   k.new_max_blocks = p->new_max_blocks_per_seq;
   k.budget = p->budget; k.sink = p->sink_tokens; k.recent = p->recent_tokens;
+  k.dependent_launch = g_env.dependent_launch;
   const cudaError_t e = launch_kv_evict(k, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail("kv evict launch", e);
   g_launches += 2;

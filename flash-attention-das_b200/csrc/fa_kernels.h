@@ -250,6 +250,12 @@ struct PageSelectParams {
   int32_t b, sq, h, h_k, group, d, page_size, num_blocks, max_blocks;
   int32_t num_pages, sink_pages, recent_pages;
   void* workspace;
+  int32_t dependent_launch;  // launch with programmatic stream serialisation (the kernels wait by themselves)
+  // set by launch_page_select
+  uint64_t* wide;            // [b * h_k][max_blocks]
+  float* scores;             // [b * h_k][max_blocks]
+  float* errors;             // [b * h_k][err_stride]
+  int32_t err_stride, batches;
 };
 size_t page_select_workspace_bytes(int b, int h_k, int max_blocks);
 cudaError_t launch_page_select(int dtype, const PageSelectParams& p, cudaStream_t stream);
@@ -288,6 +294,7 @@ struct KvEvictParams {
   int32_t* seqlens_out;
   int32_t b, h_k, row_bytes, page_size, num_blocks, max_blocks, new_max_blocks;
   int32_t budget, sink, recent;
+  int32_t dependent_launch;  // launch with programmatic stream serialisation (the kernels wait by themselves)
 };
 cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t stream);
 

@@ -25,9 +25,14 @@ __device__ __forceinline__ int evict_len(const KvEvictParams& p, int bi, bool re
   return len;
 }
 
+// V keys in a row per thread; IN_REGS: the row's keys stay in registers (up to V * kPickThreads tokens), else they are read
+// again for every pass.
+template <int V, bool IN_REGS>
 __global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const KvEvictParams p) {
   __shared__ TopkShared sh;
   const int hk = blockIdx.x, bi = blockIdx.y, tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   const int len = evict_len(p, bi, hk == 0 && tid == 0);
   const int kept = min(len, p.budget);
   const float* w = p.w_in + bi * p.win_b + hk * p.win_h;
@@ -40,16 +45,45 @@ __global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const KvEvictP
       if (wo != w) wo[i] = w[i];
     }
   } else {
-    auto key = [&](int i) -> uint32_t { return (i < p.sink || i >= len - p.recent) ? ~0u : order_key(w[i]); };
+    auto load = [&](int i0, uint32_t (&k)[V], float (&x)[V]) {   // keys i0 .. i0 + V - 1; 0: past the end
+      if (i0 + V <= len && (reinterpret_cast<uintptr_t>(w + i0) & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(w + i0 + j);
+          x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = i0 + j < len ? w[i0 + j] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int i = i0 + j;
+        k[j] = i >= len ? 0u : ((i < p.sink || i >= len - p.recent) ? ~0u : order_key(x[j]));
+      }
+    };
+    constexpr int kTile = V * kPickThreads;
+    uint32_t k[V];
+    float x[V];
+    if (IN_REGS) load(tid * V, k, x);
     int take_equal;
-    const uint32_t border = topk_border<kPickThreads, uint32_t>(len, kept, key, sh, take_equal);
-    // the weights move with the keys, chunk by chunk: a chunk's weights are read before topk_emit's barrier inside the
-    // chunk (key) and again here, and the positions written lie at or below the ones read
-    topk_emit<kPickThreads>(len, border, take_equal, key, sh, [&](bool take, int at, int i) {
-      const float x = take ? w[i] : 0.f;
-      __syncthreads();   // every thread has read its weight
-      if (take) { out[at] = i; wo[at] = x; }
-    });
+    const uint32_t border = topk_border<kPickThreads>(kept, [&](auto f) {
+      for (int i0 = 0; i0 < len; i0 += kTile) {
+        if (!IN_REGS) load(i0 + tid * V, k, x);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f(k[j]);
+      }
+    }, sh, take_equal);
+    // the weights move with the keys, tile by tile: a tile's weights are read before topk_place's barriers, and the
+    // positions written lie at or below the ones read
+    TopkCount base;
+    for (int i0 = 0; i0 < len; i0 += kTile) {
+      if (!IN_REGS) load(i0 + tid * V, k, x);
+      topk_place<kPickThreads, V>(k, border, take_equal, base, sh, [&](int j, int at) {
+        out[at] = i0 + tid * V + j;
+        wo[at] = x[j];
+      });
+    }
     __syncthreads();
     for (int i = kept + tid; i < len; i += kPickThreads) wo[i] = 0.f;
   }
@@ -59,6 +93,8 @@ __global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const KvEvictP
 // blockIdx: x piece (one CTA walks all pieces in place), y kv head and K / V, z sequence.
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const KvEvictParams p) {
   const int hk = blockIdx.y >> 1, bi = blockIdx.z, tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   const bool is_v = blockIdx.y & 1;
   const int len = evict_len(p, bi, false);
   const int kept = min(len, p.budget);
@@ -105,13 +141,25 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const KvEvictP
 }  // namespace
 
 cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t stream) {
-  evict_pick_kernel<<<dim3(p.h_k, p.b), kPickThreads, 0, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.h_k, p.b);
+  cfg.blockDim = dim3(kPickThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.dependent_launch ? 1 : 0;
+  const int64_t most = min(static_cast<int64_t>(p.max_blocks) * p.page_size, static_cast<int64_t>(p.capacity));
+  cudaError_t e = most <= 4 * kPickThreads    ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<4, true>, p)
+                  : most <= 16 * kPickThreads ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<16, true>, p)
+                                              : cudaLaunchKernelEx(&cfg, evict_pick_kernel<8, false>, p);
   if (e != cudaSuccess) return e;
   const int piece = kMoveThreads / (p.row_bytes >> 4) * kMoveUnroll;
   const int pieces = p.new_block_table ? (p.budget + piece - 1) / piece : 1;
-  evict_move_kernel<<<dim3(pieces, p.h_k * 2, p.b), kMoveThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  cfg.gridDim = dim3(pieces, p.h_k * 2, p.b);
+  cfg.blockDim = dim3(kMoveThreads);
+  return cudaLaunchKernelEx(&cfg, evict_move_kernel, p);
 }
 
 }  // namespace fa

@@ -1,13 +1,13 @@
-// Choice of the k largest of a row's values by one CTA, ties to the lowest index: the border value by a radix search
-// over order-preserving integer keys (one histogram of 8 bits of the key per pass), then the chosen indices in
-// ascending order.  Integer counts only, so the result does not depend on the order in which threads run.
+// Choice of the k largest of a row's values by one CTA, ties to the lowest index: the border value by a histogram search
+// over order-preserving integer keys, then the chosen indices in ascending order.  Integer counts only, so the result
+// does not depend on the order in which threads run.
 #pragma once
 
 #include "fa_common.cuh"
 
 namespace fa {
 
-// Keys that compare as the values do: -0 equals +0 and every NaN is above +inf.  ~0 is above every value's key.
+// Keys that compare as the values do: -0 equals +0 and every NaN is above +inf.  ~0 is above every value's key, 0 below.
 __device__ __forceinline__ uint32_t order_key(float x) {
   uint32_t u = __float_as_uint(x);
   if ((u & 0x7fffffffu) > 0x7f800000u) u = 0x7fc00000u;
@@ -21,32 +21,152 @@ __device__ __forceinline__ uint64_t order_key(double x) {
   return (u & 0x8000000000000000ull) ? ~u : (u | 0x8000000000000000ull);
 }
 
+// The value of a key (of ~0: a NaN).
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+
+constexpr int kTopkBins = 1024;
 struct TopkShared {
-  int hist[256];
-  int bin, above;
+  int hist[kTopkBins];
   int warp_total[32];
+  uint32_t lo, hi;
+  int sure, bin, above, in_bin;
 };
 
-// Border of the `want` largest of key(0) .. key(n - 1), 1 <= want <= n: all keys above the returned one belong to them,
-// and the first `take_equal` (by index) of those equal to it.
-template <int THREADS, class Key, class KeyAt>
-__device__ __forceinline__ Key topk_border(int n, int want, KeyAt key, TopkShared& sh, int& take_equal) {
+// Sum of x over the threads before this one; `total`: over all.
+template <int THREADS>
+__device__ __forceinline__ int block_exclusive(int x, TopkShared& sh, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = x;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, upto, s);
+    if (lane >= s) upto += t;
+  }
+  __syncthreads();   // the totals of the call before have been read
+  if (lane == 31) sh.warp_total[warp] = upto;
+  __syncthreads();
+  int w = lane < THREADS / 32 ? sh.warp_total[lane] : 0;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, w, s);
+    if (lane >= s) w += t;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return (warp > 0 ? before : 0) + upto - x;
+}
+
+// Border of the `want` largest of the CTA's keys, 1 <= want <= their number: all keys above the returned one belong to
+// them, and the first `take_equal` (by index) of those equal to it.  each(f) calls f(key) for the thread's share of the
+// keys (0: no key; ~0: always taken).
+//
+// Every pass counts the keys between two bounds in kTopkBins equal steps and goes on in the step that holds the border, or
+// ends when that step's keys are all wanted.  The first bounds are the smallest and largest key, so a row whose values
+// share their leading bits costs no pass for them: keys that differ need two passes, whatever their distribution is like
+// three or four.
+template <int THREADS, class Each>
+__device__ __forceinline__ uint32_t topk_border(int want, Each each, TopkShared& sh, int& take_equal) {
+  constexpr int kPer = kTopkBins / THREADS;
+  static_assert(kPer * THREADS == kTopkBins, "whole bins per thread");
   const int tid = threadIdx.x, lane = tid & 31;
-  Key prefix = 0, mask = 0;
-  for (int shift = static_cast<int>(sizeof(Key)) * 8 - 8; shift >= 0; shift -= 8) {
+  uint32_t lo = ~0u, hi = 0u;
+  int sure = 0;
+  each([&](uint32_t k) {
+    if (k == ~0u) ++sure;
+    else if (k != 0u) { lo = min(lo, k); hi = max(hi, k); }
+  });
+  if (tid == 0) { sh.lo = ~0u; sh.hi = 0u; sh.sure = 0; }
+  __syncthreads();
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  sure = __reduce_add_sync(0xffffffffu, sure);
+  if (lane == 0) {
+    atomicMin(&sh.lo, lo);
+    atomicMax(&sh.hi, hi);
+    atomicAdd(&sh.sure, sure);
+  }
+  __syncthreads();
+  lo = sh.lo; hi = sh.hi;
+  if (want <= sh.sure) {
+    take_equal = want;
+    return ~0u;
+  }
+  want -= sh.sure;
+  while (true) {
+    const uint32_t span = hi - lo;
+    const int shift = max(0, 32 - __clz(span) - 10);   // span >> shift < kTopkBins
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) sh.hist[tid + j * THREADS] = 0;
+    __syncthreads();
+    each([&](uint32_t k) {
+      if (k >= lo && k <= hi && k != ~0u) atomicAdd(&sh.hist[(k - lo) >> shift], 1);
+    });
+    __syncthreads();
+    int own[kPer], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) { own[j] = sh.hist[kTopkBins - 1 - (tid * kPer + j)]; sum += own[j]; }
+    int above = block_exclusive<THREADS>(sum, sh, total);
+    if (above < want && want <= above + sum) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (above < want && want <= above + own[j]) { sh.bin = kTopkBins - 1 - (tid * kPer + j); sh.above = above; sh.in_bin = own[j]; }
+        above += own[j];
+      }
+    }
+    __syncthreads();
+    want -= sh.above;
+    lo += static_cast<uint32_t>(sh.bin) << shift;
+    hi = min(hi, lo + ((1u << shift) - 1u));
+    if (sh.in_bin == want) {   // every key of the step (lo > 0: a key is not 0)
+      take_equal = 0;
+      return lo - 1u;
+    }
+    if (shift == 0) {
+      take_equal = want;
+      return lo;
+    }
+  }
+}
+
+// Running numbers of the chosen.
+struct TopkCount { int gt = 0, eq = 0; };
+
+// The chosen among the next THREADS * V keys, V of them in a row per thread: emit(j, position) for the thread's chosen key j.
+// All threads call it.
+template <int THREADS, int V, class Emit>
+__device__ __forceinline__ void topk_place(const uint32_t (&k)[V], uint32_t border, int take_equal, TopkCount& base, TopkShared& sh, Emit emit) {
+  static_assert(THREADS * V <= 32768, "both counts fit a half word");
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) mine += (k[j] > border ? 1 : 0) | (k[j] == border && border != 0u ? 0x10000 : 0);
+  int total;
+  const int before = block_exclusive<THREADS>(mine, sh, total);
+  int n_gt = base.gt + (before & 0xffff), n_eq = base.eq + (before >> 16);
+  if (mine != 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const bool gt = k[j] > border, eq = k[j] == border && border != 0u;
+      if (gt || (eq && n_eq < take_equal)) emit(j, n_gt + min(n_eq, take_equal));
+      n_gt += gt ? 1 : 0;
+      n_eq += eq ? 1 : 0;
+    }
+  }
+  base.gt += total & 0xffff;
+  base.eq += total >> 16;
+}
+
+// The same border search over 64-bit keys, eight bits at a time: the rare rows whose choice 32 bits do not settle.
+// each(f) calls f(key, valid) the same number of times in every thread of a warp.
+template <int THREADS, class Each>
+__device__ __noinline__ uint64_t topk_border64(int want, Each each, TopkShared& sh, int& take_equal) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  uint64_t prefix = 0, mask = 0;
+  for (int shift = 56; shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += THREADS) sh.hist[i] = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += THREADS) {
-      const int i = i0 + tid;
-      int digit = 256;
-      if (i < n) {
-        const Key x = key(i);
-        if ((x & mask) == prefix) digit = static_cast<int>((x >> shift) & 255);
-      }
-      // values of one row share their leading bits: count equal digits of a warp with one atomic
-      const uint32_t peers = __match_any_sync(0xffffffffu, digit);
-      if (digit < 256 && lane == __ffs(peers) - 1) atomicAdd(&sh.hist[digit], __popc(peers));
-    }
+    each([&](uint64_t x, bool valid) {
+      if (valid && (x & mask) == prefix) atomicAdd(&sh.hist[(x >> shift) & 255], 1);
+    });
     __syncthreads();
     if (tid < 32) {   // lane l looks at digits 255 - 8 l .. 248 - 8 l
       int own[8], sum = 0;
@@ -68,48 +188,13 @@ __device__ __forceinline__ Key topk_border(int n, int want, KeyAt key, TopkShare
       }
     }
     __syncthreads();
-    prefix |= static_cast<Key>(sh.bin) << shift;
-    mask |= static_cast<Key>(255) << shift;
+    prefix |= static_cast<uint64_t>(sh.bin) << shift;
+    mask |= 255ull << shift;
     want -= sh.above;
     __syncthreads();
   }
   take_equal = want;
   return prefix;
-}
-
-// Calls emit(position, i) for the chosen indices i in ascending order (position 0, 1, ..) and rest(i) for the others.
-// emit's reads of a chunk's values are the caller's business: `chunk_sync` barriers separate the chunks.
-template <int THREADS, class Key, class KeyAt, class Emit>
-__device__ __forceinline__ void topk_emit(int n, Key border, int take_equal, KeyAt key, TopkShared& sh, Emit emit) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int base_gt = 0, base_eq = 0;
-  for (int i0 = 0; i0 < n; i0 += THREADS) {
-    const int i = i0 + tid;
-    bool gt = false, eq = false;
-    if (i < n) {
-      const Key x = key(i);
-      gt = x > border;
-      eq = x == border;
-    }
-    const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) sh.warp_total[warp] = __popc(bg) | (__popc(be) << 16);
-    __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-      const int t = sh.warp_total[w];
-      if (w < warp) before += t;
-      total += t;
-    }
-    const uint32_t below = (1u << lane) - 1u;
-    const int n_gt = base_gt + (before & 0xffff) + __popc(bg & below);
-    const int n_eq = base_eq + (before >> 16) + __popc(be & below);
-    const bool chosen = gt || (eq && n_eq < take_equal);
-    emit(chosen, n_gt + min(n_eq, take_equal), i);
-    base_gt += total & 0xffff;
-    base_eq += total >> 16;
-    __syncthreads();
-  }
 }
 
 }  // namespace fa

@@ -1375,18 +1375,16 @@ def page_select(q, bounds, block_table, cache_seqlens, page_size, num_pages, sin
     p.num_pages, p.sink_pages, p.recent_pages = num_pages, sink_pages, recent_pages
     p.dtype = _DT[q.dtype]
     _require(num_pages > 0, "page_select: num_pages must be positive")
-    # one allocation: the two tables and the lengths
-    n = b * h_k * num_pages
-    buf = torch.empty(2 * n + b * h_k, dtype=torch.int32, device=q.device)
-    p.page_table = buf.data_ptr()
-    p.page_index = p.page_table + 4 * n
-    p.seqlens_out = p.page_table + 8 * n
+    both = torch.empty((2, b, h_k, num_pages), dtype=torch.int32, device=q.device)
+    table, index = both.unbind(0)
+    lens = torch.empty((b, h_k), dtype=torch.int32, device=q.device)
+    p.page_table, p.page_index, p.seqlens_out = table.data_ptr(), index.data_ptr(), lens.data_ptr()
     with _on_device(q.device):
         ws = _workspace(q.device, int(_lib.fa_b200_page_select_workspace_bytes(ctypes.byref(p))))
         if ws is not None:
             p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
         _check(_lib.fa_b200_page_select(ctypes.byref(p), _stream(q)), "page_select")
-    return buf[:n].view(b, h_k, num_pages), buf[2 * n:].view(b, h_k), buf[n:2 * n].view(b, h_k, num_pages)
+    return table, lens, index
 
 
 def decode_budget(q, kcache, vcache, block_table, seqlens, softmax_scale, is_causal=False, out=None, s_aux=None,
@@ -1505,13 +1503,12 @@ def kv_evict(k_cache, v_cache, block_table, cache_seqlens, weights, budget, sink
     p.page_size, p.num_blocks, p.max_blocks_per_seq = page, nb, block_table.shape[1]
     p.budget, p.sink_tokens, p.recent_tokens = budget, sink_tokens, recent_tokens
     p.dtype = _DT_CACHE[k_cache.dtype]
-    n = b * h_k * budget
-    buf = torch.empty(n + b, dtype=torch.int32, device=dev)
-    p.kept_index = buf.data_ptr()
-    p.seqlens_out = p.kept_index + 4 * n
+    kept = torch.empty((b, h_k, budget), dtype=torch.int32, device=dev)
+    lens = torch.empty((b,), dtype=torch.int32, device=dev)
+    p.kept_index, p.seqlens_out = kept.data_ptr(), lens.data_ptr()
     with _on_device(dev):
         _check(_lib.fa_b200_kv_evict(ctypes.byref(p), _stream(k_cache)), "kv_evict")
-    return buf[:n].view(b, h_k, budget), buf[n:]
+    return kept, lens
 
 
 # ------------------------------------------------------------------------------------------------
