@@ -1196,13 +1196,14 @@ int fa_b200_page_select(const fa_b200_page_select_params* p, void* stream) {
   return FA_B200_OK;
 }
 
-// Shares of the query tiles per key tile: enough CTAs for about four rounds of the 296 CTA slots (148 SMs x 2; under a
-// causal mask a CTA's work runs from all query tiles to one), as long as a share keeps at least eight tiles.
+// Shares of the query tiles per key tile: enough items for twelve rounds of the CTA slots (148 SMs x 2 up to d = 128; under a
+// causal mask an item's work runs from all query tiles to one), as long as a share keeps at least eight tiles.
 static int token_weights_chunks(const fa_b200_token_weights_params* p, int max_len) {
   const int tt = 128 / (p->h / p->h_k);
-  const int64_t ctas = static_cast<int64_t>((max_len + 127) / 128) * p->h_k * p->b;
-  const int64_t tiles = (p->max_seqlen_q + tt - 1) / tt;
-  int64_t c = ctas > 0 ? (1184 + ctas - 1) / ctas : 1;
+  const int keys = token_weights_item_keys(p->d);
+  const int64_t items = static_cast<int64_t>((max_len + keys - 1) / keys) * p->h_k * p->b, slots = p->d > 128 ? 148 : 296;
+  const int64_t tiles = (static_cast<int64_t>(p->max_seqlen_q) + tt - 1) / tt;
+  int64_t c = items > 0 ? (12 * slots + items - 1) / items : 1;
   if (c > tiles / 8) c = tiles / 8;
   if (c > 16) c = 16;
   return c < 1 ? 1 : static_cast<int>(c);
@@ -1273,6 +1274,11 @@ int fa_b200_token_weights(const fa_b200_token_weights_params* p, void* stream) {
   k.scale_log2 = p->softmax_scale * kLog2e;
   k.total_q = p->total_q;
   k.num_chunks = token_weights_chunks(p, max_len);
+  if (static_cast<int64_t>((max_len + 127) / 128) * p->h_k * k.num_chunks * p->b > 0x7fff0000) return FA_B200_ERR_TOO_LARGE;
+  k.max_q = p->max_seqlen_q;
+  k.item_keys = token_weights_item_keys(p->d);
+  k.resident = p->max_seqlen_q <= k.tile_tokens ? 1 : 0;
+  k.dependent_launch = g_env.dependent_launch;
   k.partial = static_cast<float*>(p->workspace);
   k.partial_stride = max_len;
   const cudaError_t e = launch_token_weights(p->dtype, tq, tk, k, static_cast<cudaStream_t>(stream));

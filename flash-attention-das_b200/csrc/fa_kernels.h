@@ -316,10 +316,15 @@ struct TokenWeightsParams {
   float scale_log2;
   int32_t tile_tokens;       // query tokens in a tile: its rows are tile_tokens x group
   int64_t total_q;
+  int32_t item_keys;         // keys of a work item: token_weights_item_keys(d)
+  int32_t max_q;             // longer query ranges are reported and left out
+  int32_t resident;          // every sequence has one query tile at most
   int32_t num_chunks;        // query tiles are split into num_chunks interleaved shares per key tile
+  int32_t dependent_launch;  // launch with programmatic stream serialisation (the kernels wait by themselves)
   float* partial;            // [num_chunks][b][h_k][partial_stride], when num_chunks > 1
   int64_t partial_stride;
 };
+int token_weights_item_keys(int d);
 cudaError_t launch_token_weights(int dtype, const CUtensorMap& tmap_q, const CUtensorMap& tmap_k, const TokenWeightsParams& p,
                                  cudaStream_t stream);
 

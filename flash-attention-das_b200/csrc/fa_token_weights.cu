@@ -5,16 +5,23 @@
 // log-sum-exp is known this kernel reads them back: w[t] = decay w[t] + sum_r 2^(s_rt - lse_r), rows in a fixed order.
 //
 // Of a prompt.  Given every query's log-sum-exp the weight of key t is a plain sum over the queries, with no running
-// maximum: a CTA owns 128 keys of one kv head, keeps their tile in shared memory as the A operand and walks the query
-// tiles that see them, S^T = K Q^T in TMEM.  A TMEM lane is then a key, so a key's sum stays in one thread's register:
-// no reduction between threads, no atomics, no second pass.  A query tile holds 128 / group tokens of all heads of the
-// group (rows token-major), which fills it for short windows too and makes the causal mask a column bound per key.
-//   warps 0-3  one thread per key: 2^(s - lse) and its sum
-//   warp 4     TMA producer: the key tile once (through the block table), query tiles into a ring
-//   warp 5     MMA issuer, two S^T buffers
+// maximum: a CTA takes 128 keys of one kv head (256 above d = 128) as the A operand and walks the query tiles that see them,
+// S^T = K Q^T in TMEM.  A TMEM lane is then a key, so a key's sum stays in a thread's registers: no atomics, no second pass.
+// A query tile holds 128 / group tokens of all heads of the group (rows token-major), which fills it for short windows too
+// and makes the causal mask a column bound per key.
+//   warps 0-7  one thread per key and half of a tile's columns (above d = 128: per key of 256): 2^(s - lse) and its sum
+//   warp 8     TMA producer: key tiles (through the block table) and query tiles into a pool of tile buffers
+//   warp 9     MMA issuer, two S^T buffers per 128 keys
+// Two persistent CTAs per SM (one above d = 128) walk the items (key tiles, kv head, share of the query tiles) of the batch,
+// so that the loads and the first product of an item run during the sums of the one before.  Long prompts: items go round
+// robin, heaviest first under a causal mask, and a key tile's query tiles are cut into shares (every num_chunks-th tile),
+// whose sums a small kernel adds in order.  Short windows (one query tile per sequence): a CTA takes consecutive key tiles
+// and keeps the query tile, which leaves the keys as the only traffic.
+//
 // Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit, its tcgen05 product 256.
-// Long prompts are cut into shares of the query tiles per key tile (every num_chunks-th tile), whose sums a small kernel
-// adds in order.
+// One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128, causal): 397 us, 69 % of what the MUFU units could do at the
+// 1.7 GHz that the GPU ran at.  One CTA per SM with 256 keys, which halves the query traffic, measured 536 us, eight warps per SM
+// instead of sixteen 436 us, a CTA per key tile 424 us.  32 queries against 4 x 16384 keys: a CTA per key tile 78 us.
 #include "fa_prefill_common.cuh"
 
 namespace fa {
@@ -50,39 +57,80 @@ __global__ void __launch_bounds__(kFinishThreads) weights_finish_kernel(const We
   p.w_out[bi * p.wout_b + hk * p.wout_h + tok] = before + sum;
 }
 
-constexpr int kTwThreads = 192;
-constexpr int kTwSlots = 2;
-struct TwLayout { int q_off, lse_off, bar_off, misc_off, total; };
+// 128-key halves of a CTA: two CTAs per SM with one up to d = 128, one CTA with two above (shared memory).  Eight warps take
+// the sums either way: with one half, two warps share 32 keys and take half of a tile's columns each (16 warps per SM keep the
+// MUFU unit busier than 8 do).
+__host__ __device__ constexpr int tw_halves(int hd) { return hd > 128 ? 2 : 1; }
+constexpr int kTwThreads = 320;
+constexpr int kTwMaxTiles = 6;
+// Tile buffers for keys and queries.
+__host__ __device__ constexpr int tw_tiles(int hd) { return hd == 64 ? 6 : (hd == 192 ? 4 : 3); }
+struct TwLayout { int lse_off, bar_off, misc_off, total; };
 template <int DT, int HD>
 __host__ __device__ constexpr TwLayout tw_layout() {
   TwLayout s{};
-  s.q_off = TileTraits<DT, HD>::kTileBytes;
-  s.lse_off = s.q_off + kTwSlots * TileTraits<DT, HD>::kTileBytes;
-  s.bar_off = s.lse_off + 2 * 128 * 4;
-  s.misc_off = s.bar_off + 8 * (1 + 2 * kTwSlots + 4);
+  s.lse_off = tw_tiles(HD) * TileTraits<DT, HD>::kTileBytes;
+  s.bar_off = s.lse_off + 8 * 2 * 128 * 4 + 2 * 128 * 4;
+  s.misc_off = s.bar_off + 8 * (2 * kTwMaxTiles + 8);
   s.total = s.misc_off + 16;
   return s;
 }
 
-// Sum of 2^(scale s + neg_lse) over the columns [c_first, c_end) of one S^T row; MASK false: all 128 columns.  `release`
-// runs once the row has been read from TMEM.
-template <bool MASK, class Release>
+// Groups of four columns, of the eight in 32, whose exponentials go to the FMA pipe instead of the MUFU unit.  Measured on one
+// prompt of 8192 tokens (32 heads, 8 kv heads, bf16): none 408 us, one group 397, two 416, three 444: the kernel is bound by
+// the instructions it issues nearly as much as by the MUFU unit.
+constexpr int kPolyGroups = 0x10;
+// 2^x of two values on the FMA pipe: round-to-nearest range reduction by the magic-number add, a degree-5 polynomial of 2^f
+// on [-0.5, 0.5] (weighted least squares towards the minimax, constant term 1; relative error 9.2e-8, 1.7e-7 with its 32-bit
+// rounding), the integer part added to the exponent field.  x is clamped to [-127, 128], where that gives exactly 0 and
+// infinity: with the constant term 1 no mantissa falls below 1 at the lower end.
+__device__ __forceinline__ void exp2_poly2(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  unpack_f32x2(x, x0, x1);
+  x0 = fminf(fmaxf(x0, -127.f), 128.f);
+  x1 = fminf(fmaxf(x1, -127.f), 128.f);
+  const uint64_t x2 = pack_f32x2(x0, x1);
+  const uint64_t t2 = add_f32x2(x2, pack_f32x2(12582912.f, 12582912.f));   // 1.5 * 2^23: the low mantissa bits hold round(x)
+  const uint64_t r2 = add_f32x2(t2, pack_f32x2(-12582912.f, -12582912.f));
+  const uint64_t f2 = fma_f32x2(r2, pack_f32x2(-1.f, -1.f), x2);
+  uint64_t q2 = fma_f32x2(f2, pack_f32x2(0.001326472731307149f, 0.001326472731307149f), pack_f32x2(0.009671512991189957f, 0.009671512991189957f));
+  q2 = fma_f32x2(q2, f2, pack_f32x2(0.05550733581185341f, 0.05550733581185341f));
+  q2 = fma_f32x2(q2, f2, pack_f32x2(0.24022242426872253f, 0.24022242426872253f));
+  q2 = fma_f32x2(q2, f2, pack_f32x2(0.6931470036506653f, 0.6931470036506653f));
+  q2 = fma_f32x2(q2, f2, pack_f32x2(1.f, 1.f));
+  float q0, q1, t0, t1;
+  unpack_f32x2(q2, q0, q1);
+  unpack_f32x2(t2, t0, t1);
+  p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
+  p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
+}
+
+// Sum of 2^(scale s + neg_lse) over the columns [c_first, c_end) of COLS columns of an S^T row; MASK false: all of them.
+// `release` runs once the row has been read from TMEM.
+template <bool MASK, int COLS, class Release>
 __device__ __forceinline__ float tile_sum(uint32_t t_s, const float* neg_lse, float scale, int c_first, int c_end, Release release) {
   const uint64_t sc2 = pack_f32x2(scale, scale);
   uint64_t acc0 = 0ull, acc1 = 0ull;
-#pragma unroll
-  for (int ch = 0; ch < 4; ++ch) {
-    uint32_t s[32];
-    tmem_ld_32x32(t_s + ch * 32, s);
+#pragma unroll 1
+  for (int ch = 0; ch < COLS / 32; ++ch) {   // a loop, for the instruction cache
+    uint32_t v[32];
+    tmem_ld_32x32(t_s + ch * 32, v);
     tmem_wait_ld();
-    if (ch == 3) release();
+    if (ch == COLS / 32 - 1) release();
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       const float4 l = *reinterpret_cast<const float4*>(neg_lse + ch * 32 + i);
+      const uint64_t xa = fma_f32x2(pack_f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, pack_f32x2(l.x, l.y));
+      const uint64_t xb = fma_f32x2(pack_f32x2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2, pack_f32x2(l.z, l.w));
       float x0, x1, x2, x3;
-      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, pack_f32x2(l.x, l.y)), x0, x1);
-      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), sc2, pack_f32x2(l.z, l.w)), x2, x3);
-      x0 = fast_exp2(x0); x1 = fast_exp2(x1); x2 = fast_exp2(x2); x3 = fast_exp2(x3);
+      if (!MASK && ((kPolyGroups >> (i / 4)) & 1)) {
+        exp2_poly2(xa, x0, x1);
+        exp2_poly2(xb, x2, x3);
+      } else {
+        unpack_f32x2(xa, x0, x1);
+        unpack_f32x2(xb, x2, x3);
+        x0 = fast_exp2(x0); x1 = fast_exp2(x1); x2 = fast_exp2(x2); x3 = fast_exp2(x3);
+      }
       if (MASK) {   // a column that holds no visible query may hold anything
         const int c = ch * 32 + i;
         x0 = (c >= c_first && c < c_end) ? x0 : 0.f;
@@ -100,180 +148,390 @@ __device__ __forceinline__ float tile_sum(uint32_t t_s, const float* neg_lse, fl
   return (a + b) + (c + d);
 }
 
-// A barrier that a copy in flight will still complete: waited for after an abort, with a limit, so that nothing writes
-// into shared memory that the CTA has given back.
+// A barrier that a copy or product in flight will still complete: waited for after an abort, with a limit, so that nothing
+// writes into memory that the CTA has given back.
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < (1 << 16) && !mbar_try_wait(bar, parity); ++i) {}
 }
 
-// blockIdx: x share of the query tiles and kv head, y key tile (causal: heaviest first), z sequence.
+// The sequence's tokens and queries as every role of the kernel sees them.
+struct TwSeq { int len, q0, n, tiles; };
+__device__ __forceinline__ TwSeq tw_seq(const TokenWeightsParams& p, int b) {
+  TwSeq s;
+  s.len = min(max(p.seqlens[b], 0), p.max_len);
+  s.q0 = p.cu_q[b];
+  s.n = p.cu_q[b + 1] - s.q0;
+  if (s.n < 0 || s.n > p.max_q || s.q0 < 0 || static_cast<int64_t>(s.q0) + s.n > p.total_q) s.n = 0;   // reported by tw_report
+  s.tiles = (s.n + p.tile_tokens - 1) / p.tile_tokens;
+  return s;
+}
+
+// One CTA's walk over its items and their query tiles.  KEYS: keys of an item.
+template <int KEYS>
+struct TwWalk {
+  int item, end, stride;         // items left
+  int b, base, here;             // sequence, its first item, its number of items
+  int key_tiles;
+  TwSeq s;
+  int hk, chunk, k0, first, steps, j;
+  __device__ __forceinline__ void enter(const TokenWeightsParams& p, int sequence) {
+    b = sequence;
+    s = tw_seq(p, b);
+    key_tiles = (s.len + KEYS - 1) / KEYS;
+    here = key_tiles * p.h_k * p.num_chunks;
+  }
+  // Moves to the next query tile, or the next item (steps may be 0: no query sees its keys).  false: done.
+  __device__ __forceinline__ bool next(const TokenWeightsParams& p) { return ++j < steps || next_item(p); }
+  __device__ __forceinline__ bool next_item(const TokenWeightsParams& p) {
+    item += stride;
+    if (item >= end) return false;
+    while (item >= base + here) {
+      base += here;
+      enter(p, b + 1);
+    }
+    int i = item - base;
+    int kt;
+    if (p.resident) {              // one query tile: key tiles innermost
+      hk = i / key_tiles;
+      kt = i - hk * key_tiles;
+      chunk = 0;
+    } else {                       // key tiles outermost: heaviest first under a causal mask
+      const int per = p.h_k * p.num_chunks;
+      kt = i / per;
+      i -= kt * per;
+      hk = p.num_chunks > 1 ? i / p.num_chunks : i;
+      chunk = i - hk * p.num_chunks;
+    }
+    k0 = kt * KEYS;
+    const int shift = s.len - s.n;                                   // query i sits at position shift + i
+    first = ((p.causal && k0 > shift) ? (k0 - shift) / p.tile_tokens : 0) + chunk;
+    steps = max(s.tiles - first, 0);
+    if (p.num_chunks > 1) steps = (steps + p.num_chunks - 1) / p.num_chunks;
+    j = 0;
+    return true;
+  }
+  __device__ __forceinline__ bool begin(const TokenWeightsParams& p, int total) {
+    if (p.resident) {              // a contiguous share
+      const int64_t g = gridDim.x;
+      item = static_cast<int>(total * static_cast<int64_t>(blockIdx.x) / g) - 1;
+      end = static_cast<int>(total * static_cast<int64_t>(blockIdx.x + 1) / g);
+      stride = 1;
+    } else {
+      item = static_cast<int>(blockIdx.x) - static_cast<int>(gridDim.x);
+      end = total;
+      stride = gridDim.x;
+    }
+    base = 0; steps = 0; j = 0;
+    enter(p, 0);
+    return next_item(p);
+  }
+  __device__ __forceinline__ int tile_token(const TokenWeightsParams& p) const { return (first + j * p.num_chunks) * p.tile_tokens; }
+  // Whether the second 128 keys exist, and whether a query of this tile sees one of them.
+  __device__ __forceinline__ bool second() const { return KEYS > 128 && k0 + 128 < s.len; }
+  __device__ __forceinline__ bool active(const TokenWeightsParams& p, int half) const {
+    if (steps == 0) return false;
+    if (half == 0) return true;
+    return second() && (!p.causal || tile_token(p) + p.tile_tokens > k0 + 128 - (s.len - s.n));
+  }
+};
+
+// Tile buffers as producer and MMA issuer both go through them: a load takes the buffer whose last use lies furthest back
+// (keys are used until their item's last step, a resident query tile until the kv head changes).
+template <int N>
+struct TwBuffers {
+  int last[N], loads[N];
+  __device__ __forceinline__ TwBuffers() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) { last[i] = -1; loads[i] = 0; }
+  }
+  __device__ __forceinline__ int take(int until) {
+    int s = 0, least = last[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+      if (last[i] < least) { s = i; least = last[i]; }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i == s) { last[i] = until; ++loads[i]; }
+    return s;
+  }
+  __device__ __forceinline__ int count(int s) const {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n = i == s ? loads[i] : n;
+    return n;
+  }
+  __device__ __forceinline__ void ends(int s, int at) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i == s) last[i] = at;
+  }
+};
+
 template <int DT, int HD>
 __global__ void __launch_bounds__(kTwThreads, HD > 128 ? 1 : 2)
 token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const TokenWeightsParams p) {
   using T = TileTraits<DT, HD>;
   constexpr TwLayout L = tw_layout<DT, HD>();
+  constexpr int kTiles = tw_tiles(HD), kHalvesOfKeys = tw_halves(HD), kProducer = 8, kMma = 9;
+  constexpr int kSplit = 2 / kHalvesOfKeys, kColsOfWarp = 128 / kSplit, kLaneCols = kColsOfWarp / 32;
+  constexpr int kCols = 256 * kHalvesOfKeys;   // TMEM
+  constexpr int kForever = 0x7fffffff;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sm_lse = reinterpret_cast<float*>(smem + L.lse_off);          // [2][128], minus lse in log2 units
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L.bar_off);
-  uint64_t* q_full = k_full + 1;
-  uint64_t* q_empty = q_full + kTwSlots;
-  uint64_t* s_full = q_empty + kTwSlots;   // [2]
-  uint64_t* s_empty = s_full + 2;          // [2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bar_off);   // [kTiles]
+  uint64_t* empty = full + kTwMaxTiles;                             // [kTiles]
+  uint64_t* s_full = empty + kTwMaxTiles;                           // [2 halves][2]
+  uint64_t* s_empty = s_full + 4;                                   // [2 halves][2]
   uint32_t* sm_tmem_base = reinterpret_cast<uint32_t*>(smem + L.misc_off);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L.misc_off + 4);
+  int* sm_total = reinterpret_cast<int*>(smem + L.misc_off + 8);
   const WaitCtx wctx{abort_flag, p.status};
-
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.x / p.num_chunks, chunk = blockIdx.x - hk * p.num_chunks;
-  const int k0 = blockIdx.y * 128, bi = blockIdx.z;
-  int len = p.seqlens[bi];
-  if (len > p.max_len) {
-    len = p.max_len;
-    if (threadIdx.x == 0) atomicOr(p.status, kRangeBit);
-  }
-  if (k0 >= len) return;
-  const int q0 = p.cu_q[bi];
-  int n = p.cu_q[bi + 1] - q0;
-  if (n < 0 || q0 < 0 || static_cast<int64_t>(q0) + n > p.total_q) {
-    n = 0;
-    if (threadIdx.x == 0) atomicOr(p.status, kRangeBit);
-  }
-  const int shift = len - n;                                            // query i sits at position shift + i
-  const int tt = p.tile_tokens;
-  const int first = (p.causal && k0 > shift) ? (k0 - shift) / tt : 0;   // first query tile that sees a key of this tile
-  const int tiles = (n + tt - 1) / tt;
-  const int steps = tiles - first > chunk ? (tiles - first - chunk + p.num_chunks - 1) / p.num_chunks : 0;
-  const int key = k0 + threadIdx.x;                                     // warps 0-3
-  float sum = 0.f, comp = 0.f;
-  bool ok = true;
 
-  if (steps > 0) {
-    if (threadIdx.x == 128) {
-      *abort_flag = 0;
-      mbar_init(smem_u32(k_full), 1);
-      for (int i = 0; i < kTwSlots; ++i) {
-        mbar_init(smem_u32(&q_full[i]), 1);
-        mbar_init(smem_u32(&q_empty[i]), 1);
-      }
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(smem_u32(&s_full[i]), 1);
-        mbar_init(smem_u32(&s_empty[i]), 128);
-      }
-      mbar_fence_init();
-      tma_prefetch_desc(&tmap_q);
-      tma_prefetch_desc(&tmap_k);
+  griddep_wait();
+  griddep_launch_dependents();
+  if (threadIdx.x == 32 * kProducer) {
+    *abort_flag = 0;
+    for (int i = 0; i < kTiles; ++i) {
+      mbar_init(smem_u32(&full[i]), 1);
+      mbar_init(smem_u32(&empty[i]), 1);
     }
-    if (warp == 5) {
-      tmem_alloc(smem_u32(sm_tmem_base), 256);
-      tmem_relinquish();
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&s_empty[i]), 128 * kSplit);
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *sm_tmem_base;
-    const uint32_t k_smem = smem_u32(smem), q_smem = smem_u32(smem + L.q_off);
-    if (warp == 4) {
-      if (lane == 0) {
-        const int nbox = min(128 / p.box_rows, (len - k0 + p.box_rows - 1) / p.box_rows);
-        mbar_expect_tx(smem_u32(k_full), static_cast<uint32_t>(nbox) * p.box_rows * 128u * T::kHalves);
-        const int32_t* bt = p.block_table + bi * p.bt_stride;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+  }
+  if (warp == kMma) {
+    tmem_alloc(smem_u32(sm_tmem_base), kCols);
+    tmem_relinquish();
+  }
+  if (warp == 0) {   // number of items of the batch; what is wrong with the lengths on the device is reported once
+    int total = 0;
+    for (int b = lane; b < p.b; b += 32) {
+      const TwSeq s = tw_seq(p, b);
+      total += (s.len + 128 * kHalvesOfKeys - 1) / (128 * kHalvesOfKeys) * p.h_k * p.num_chunks;
+      const int n = p.cu_q[b + 1] - p.cu_q[b];
+      if (blockIdx.x == 0 && (p.seqlens[b] > p.max_len || n != s.n)) atomicOr(p.status, kRangeBit);
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    if (lane == 0) *sm_total = total;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *sm_tmem_base;
+  const int total = *sm_total;
+  const uint32_t tiles_smem = smem_u32(smem);
+
+  if (warp == kProducer) {
+    if (lane == 0) {
+      TwWalk<128 * kHalvesOfKeys> w{};
+      TwBuffers<kTiles> buf;
+      int t = 0, q_key = -1, q_slot = 0;     // step; (sequence, kv head) of the resident query tile
+      const uint32_t q_bytes = static_cast<uint32_t>(p.tile_tokens) * p.group * 128u * T::kHalves;
+      bool ok = true;
+      auto reserve = [&](int until) -> int {
+        const int slot = buf.take(until), n = buf.count(slot);
+        if (n > 1 && !mbar_wait(smem_u32(&empty[slot]), n & 1, wctx)) ok = false;
+        return slot;
+      };
+      auto load_keys = [&](int k0) {
+        const int slot = reserve(t + w.steps - 1);
+        if (!ok) return;
+        const uint32_t bar = smem_u32(&full[slot]);
+        const int nbox = min(128 / p.box_rows, (w.s.len - k0 + p.box_rows - 1) / p.box_rows);
+        mbar_expect_tx(bar, static_cast<uint32_t>(nbox) * p.box_rows * 128u * T::kHalves);
+        const int32_t* bt = p.block_table + w.b * p.bt_stride;
         for (int i = 0; i < nbox; ++i) {
           const int tok = k0 + i * p.box_rows;
           const int page = bt[tok / p.page_size], row = tok % p.page_size;
           for (int hf = 0; hf < T::kHalves; ++hf)
-            tma_load_4d(k_smem + hf * T::kHalfBytes + i * p.box_rows * 128, &tmap_k, smem_u32(k_full), hf * 64, hk, row, page);
+            tma_load_4d(tiles_smem + slot * T::kTileBytes + hf * T::kHalfBytes + i * p.box_rows * 128, &tmap_k, bar, hf * 64, w.hk, row, page);
         }
-        const uint32_t q_bytes = static_cast<uint32_t>(tt) * p.group * 128u * T::kHalves;
-        int j = 0;
-        for (; j < steps; ++j) {
-          const int slot = j % kTwSlots;
-          if (!mbar_wait(smem_u32(&q_empty[slot]), ((j / kTwSlots) & 1) ^ 1u, wctx)) break;
-          const uint32_t bar = smem_u32(&q_full[slot]);
-          mbar_expect_tx(bar, q_bytes);
-          const int tok = q0 + (first + chunk + j * p.num_chunks) * tt;
-          for (int hf = 0; hf < T::kHalves; ++hf)
-            tma_load_4d(q_smem + slot * T::kTileBytes + hf * T::kHalfBytes, &tmap_q, bar, hf * 64, hk * p.group, tok, 0);
-        }
-        if (j < steps) {   // gave up: the loads issued last may still be on their way
-          drain(smem_u32(k_full), 0);
-          for (int i = max(0, j - kTwSlots); i < j; ++i) drain(smem_u32(&q_full[i % kTwSlots]), (i / kTwSlots) & 1);
-        }
-      }
-    } else if (warp == 5) {
-      if (lane == 0) {
-        bool go = mbar_wait(smem_u32(k_full), 0, wctx);
-        int j = 0;
-        for (; go && j < steps; ++j) {
-          const int slot = j % kTwSlots, buf = j & 1;
-          if (!mbar_wait(smem_u32(&q_full[slot]), (j / kTwSlots) & 1, wctx)) break;
-          if (!mbar_wait(smem_u32(&s_empty[buf]), ((j >> 1) & 1) ^ 1u, wctx)) break;
-          tc_fence_after();
-          issue_qk<DT, HD>(k_smem, q_smem + slot * T::kTileBytes, tmem_base + buf * 128);   // rows: keys, columns: queries
-          tc_commit(smem_u32(&q_empty[slot]));
-          tc_commit(smem_u32(&s_full[buf]));
-        }
-        if (j < steps)     // gave up: products in flight end before TMEM is freed
-          for (int i = max(0, j - 2); i < j; ++i) drain(smem_u32(&s_full[i & 1]), (i >> 1) & 1);
-      }
-      __syncwarp();
-    } else {
-      // this thread's column of every tile: token t_in of the tile, head h_in of the group
-      const int t_in = threadIdx.x / p.group, h_in = threadIdx.x - t_in * p.group;
-      const float* lse = p.lse + (static_cast<int64_t>(hk) * p.group + h_in) * p.lse_h + q0;
-      const uint32_t t_s = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
-      auto fetch = [&](int j) -> float {
-        const int tok = (first + chunk + j * p.num_chunks) * tt + t_in;
-        return (t_in < tt && tok < n) ? -__ldg(lse + tok) * kLog2e : -INFINITY;
       };
-      float next = fetch(0);
-      for (int j = 0; j < steps; ++j) {
-        const int buf = j & 1;
-        sm_lse[buf * 128 + threadIdx.x] = next;
-        if (j + 1 < steps) next = fetch(j + 1);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        // after a wait that gave up the warps still meet at the barrier above, step by step
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&s_full[buf]), (j >> 1) & 1, wctx));
-        if (!ok) continue;
+      for (bool more = w.begin(p, total); more; more = w.next(p)) {
+        if (w.steps == 0) continue;
+        const int key = w.b * p.h_k + w.hk;
+        const bool load_q = !p.resident || key != q_key;
+        if (p.resident && load_q && q_key >= 0) buf.ends(q_slot, t - 1);
+        if (w.j == 0) {
+          load_keys(w.k0);
+          if (ok && w.second()) load_keys(w.k0 + 128);
+        }
+        if (ok && load_q) {
+          q_key = key;
+          q_slot = reserve(p.resident ? kForever : t);
+          if (ok) {
+            const uint32_t bar = smem_u32(&full[q_slot]);
+            mbar_expect_tx(bar, q_bytes);
+            for (int hf = 0; hf < T::kHalves; ++hf)
+              tma_load_4d(tiles_smem + q_slot * T::kTileBytes + hf * T::kHalfBytes, &tmap_q, bar, hf * 64, w.hk * p.group,
+                          w.s.q0 + w.tile_token(p), 0);
+          }
+        }
+        if (!ok) break;
+        ++t;
+      }
+      if (!ok)   // gave up: the loads issued last may still be on their way (one reserved and not issued just runs out)
+        for (int i = 0; i < kTiles; ++i)
+          if (buf.count(i) > 0) drain(smem_u32(&full[i]), (buf.count(i) - 1) & 1);
+    }
+  } else if (warp == kMma) {
+    if (lane == 0) {
+      TwWalk<128 * kHalvesOfKeys> w{};
+      TwBuffers<kTiles> buf;
+      int t = 0, q_key = -1, k_slot[2] = {0, 0}, q_slot = 0, n_half[2] = {0, 0};
+      bool ok = true, two = false;
+      bool more = w.begin(p, total);
+      while (more && w.steps == 0) more = w.next(p);
+      while (more && ok) {
+        const int key = w.b * p.h_k + w.hk;
+        const bool load_q = !p.resident || key != q_key;
+        if (p.resident && load_q && q_key >= 0) buf.ends(q_slot, t - 1);
+        if (w.j == 0) {
+          two = w.second();
+          k_slot[0] = buf.take(t + w.steps - 1);
+          if (two) k_slot[1] = buf.take(t + w.steps - 1);
+        }
+        if (load_q) {
+          q_key = key;
+          q_slot = buf.take(p.resident ? kForever : t);
+        }
+        ok = mbar_wait(smem_u32(&full[q_slot]), (buf.count(q_slot) - 1) & 1, wctx);
+#pragma unroll
+        for (int half = 0; half < kHalvesOfKeys; ++half) {
+          if (!ok || !w.active(p, half)) continue;
+          const int n = n_half[half]++, sb = 2 * half + (n & 1);
+          ok = mbar_wait(smem_u32(&full[k_slot[half]]), (buf.count(k_slot[half]) - 1) & 1, wctx) &&
+               mbar_wait(smem_u32(&s_empty[sb]), ((n >> 1) & 1) ^ 1u, wctx);
+          if (!ok) { --n_half[half]; break; }
+          tc_fence_after();
+          issue_qk<DT, HD>(tiles_smem + k_slot[half] * T::kTileBytes, tiles_smem + q_slot * T::kTileBytes, tmem_base + sb * 128);
+          tc_commit(smem_u32(&s_full[sb]));
+        }
+        if (!ok) break;
+        const bool k_done = w.j == w.steps - 1;
+        do { more = w.next(p); } while (more && w.steps == 0);
+        if (k_done) {
+          tc_commit(smem_u32(&empty[k_slot[0]]));
+          if (two) tc_commit(smem_u32(&empty[k_slot[1]]));
+        }
+        if (!p.resident || !more || w.b * p.h_k + w.hk != q_key) tc_commit(smem_u32(&empty[q_slot]));
+        ++t;
+      }
+      if (!ok)     // gave up: products in flight end before TMEM is freed
+        for (int half = 0; half < kHalvesOfKeys; ++half)
+          for (int i = max(0, n_half[half] - 2); i < n_half[half]; ++i) drain(smem_u32(&s_full[2 * half + (i & 1)]), (i >> 1) & 1);
+    }
+    __syncwarp();
+  } else {
+    // key half * 128 + row of the item's, columns col0 .. of every tile
+    const int half = kSplit == 1 ? warp >> 2 : 0, row = threadIdx.x & 127, col0 = kSplit == 1 ? 0 : (warp >> 2) * kColsOfWarp;
+    // this lane's columns, whose log-sum-exp it fetches for the warp: token and head
+    int t_in[kLaneCols];
+    int64_t h_off[kLaneCols];
+#pragma unroll
+    for (int e = 0; e < kLaneCols; ++e) {
+      const int c = col0 + lane * kLaneCols + e;
+      t_in[e] = c / p.group;
+      h_off[e] = static_cast<int64_t>(c - t_in[e] * p.group) * p.lse_h + t_in[e];
+    }
+    float* sm_lse = reinterpret_cast<float*>(smem + L.lse_off) + warp * 256;   // this warp's own: [2][128]
+    float* sm_sum = reinterpret_cast<float*>(smem + L.lse_off) + 8 * 256;      // [2][128]: sums of the second warp of a pair
+    const uint32_t t_s = tmem_base + half * 256 + col0 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    TwWalk<128 * kHalvesOfKeys> w{};
+    int t = 0, q_key = -1, items = 0;
+    bool ok = true;
+    float next[kLaneCols];       // log-sum-exp of the lane's columns in the tile to come; +inf: no query
+    const float* lse = nullptr;
+    auto fetch = [&](int tok0) {
+#pragma unroll
+      for (int e = 0; e < kLaneCols; ++e)
+        next[e] = (t_in[e] < p.tile_tokens && tok0 + t_in[e] < w.s.n) ? __ldg(lse + h_off[e] + tok0) : INFINITY;
+    };
+    for (bool more = w.begin(p, total); more; more = w.next_item(p)) {   // after an abort the pairs still meet, item by item
+      const int key = w.k0 + half * 128 + row;
+      float sum = 0.f, comp = 0.f;
+      // what the sum is added to, on its way during the steps
+      const bool adds = p.w_in && p.num_chunks == 1 && col0 == 0 && key < w.s.len && key < p.capacity;
+      const float before = adds ? p.w_in[w.b * p.win_b + w.hk * p.win_h + key] * p.decay : 0.f;
+      // the steps of this half: those whose last query sees its first key
+      int j = 0;
+      const int tile_step = p.num_chunks * p.tile_tokens;
+      if (half > 0) {
+        if (!w.second()) continue;
+        if (p.causal)
+          while (j < w.steps && w.first * p.tile_tokens + j * tile_step + p.tile_tokens <= w.k0 + 128 - (w.s.len - w.s.n)) ++j;
+      }
+      int tile0 = w.first * p.tile_tokens + j * tile_step;
+      if (j < w.steps && (!p.resident || w.b * p.h_k + w.hk != q_key)) {
+        q_key = w.b * p.h_k + w.hk;
+        lse = p.lse + static_cast<int64_t>(w.hk) * p.group * p.lse_h + w.s.q0;
+        fetch(tile0);
+      }
+      int ahead = key - (w.s.len - w.s.n) - tile0;   // this key's position relative to the tile's first query
+      for (; j < w.steps && ok; ++j, tile0 += tile_step, ahead -= tile_step) {
+        const int buf = t & 1;
+        // a log-sum-exp that is not finite goes with scores that may not be: the exponentials that keep infinities and NaN
+        bool plain = true;
+#pragma unroll
+        for (int e = 0; e < kLaneCols; ++e) {
+          plain = plain && fabsf(next[e]) < INFINITY;
+          sm_lse[buf * 128 + lane * kLaneCols + e] = -next[e] * kLog2e;
+        }
+        if (j + 1 < w.steps) fetch(tile0 + tile_step);
+        const int c_first = (p.causal ? max(0, min(ahead, p.tile_tokens)) * p.group : 0) - col0;
+        const int c_end = min(p.tile_tokens, w.s.n - tile0) * p.group - col0;
+        const bool mask = c_end < kColsOfWarp || __any_sync(0xffffffffu, c_first > 0 || !plain);
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[2 * half + buf]), (t >> 1) & 1, wctx));
+        if (!ok) break;
         tc_fence_after();
-        const int tile0 = (first + chunk + j * p.num_chunks) * tt;
-        const int c_first = p.causal ? max(0, min(key - shift - tile0, tt)) * p.group : 0;
-        const int c_end = min(tt, n - tile0) * p.group;
         auto release = [&] {
           tc_fence_before();
-          mbar_arrive(smem_u32(&s_empty[buf]));
+          mbar_arrive(smem_u32(&s_empty[2 * half + buf]));
         };
-        const bool mask = c_end < 128 || (p.causal && k0 + warp * 32 + 31 - shift - tile0 > 0);   // the warp's last key
-        const float part = mask ? tile_sum<true>(t_s + buf * 128, sm_lse + buf * 128, p.scale_log2, c_first, c_end, release)
-                                : tile_sum<false>(t_s + buf * 128, sm_lse + buf * 128, p.scale_log2, 0, 128, release);
+        const float part = mask ? tile_sum<true, kColsOfWarp>(t_s + buf * 128, sm_lse + buf * 128, p.scale_log2, c_first, c_end, release)
+                                : tile_sum<false, kColsOfWarp>(t_s + buf * 128, sm_lse + buf * 128, p.scale_log2, 0, kColsOfWarp, release);
         // up to tens of thousands of queries: the total carries its rounding errors along
-        const float total = __fadd_rn(sum, part);
+        const float now = __fadd_rn(sum, part);
         const float big = fmaxf(sum, part), small = fminf(sum, part);
-        comp = __fadd_rn(comp, __fsub_rn(small, __fsub_rn(total, big)));
-        sum = total;
+        comp = __fadd_rn(comp, __fsub_rn(small, __fsub_rn(now, big)));
+        sum = now;
+        ++t;
       }
-      __syncwarp();
+      sum += comp;
+      if constexpr (kSplit == 2) {   // the pair's second warp hands its sums over; two buffers, so one meeting per item
+        sm_sum += items++ & 1 ? -128 : 128;
+        if (col0 > 0) sm_sum[row] = sum;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+        if (col0 > 0) continue;
+        sum += sm_sum[row];
+      }
+      if (ok && key < w.s.len) {
+        if (p.num_chunks > 1)
+          p.partial[((static_cast<int64_t>(w.chunk) * p.b + w.b) * p.h_k + w.hk) * p.partial_stride + key] = sum;
+        else if (key < p.capacity)
+          p.w_out[w.b * p.wout_b + w.hk * p.wout_h + key] = before + sum;
+      }
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 5) {
-      tc_fence_after();
-      tmem_dealloc(tmem_base, 256);
-    }
+    __syncwarp();
   }
-  if (warp < 4 && ok && key < len) {
-    sum += comp;
-    if (p.num_chunks > 1) {
-      p.partial[((static_cast<int64_t>(chunk) * p.b + bi) * p.h_k + hk) * p.partial_stride + key] = sum;
-    } else if (key < p.capacity) {
-      const float before = p.w_in ? p.w_in[bi * p.win_b + hk * p.win_h + key] * p.decay : 0.f;
-      p.w_out[bi * p.wout_b + hk * p.wout_h + key] = before + sum;
-    }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kCols);
   }
 }
 
 __global__ void __launch_bounds__(256) token_weights_join_kernel(const TokenWeightsParams p) {
   const int hk = blockIdx.y, bi = blockIdx.z, key = blockIdx.x * 256 + threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   if (key >= min(min(p.seqlens[bi], p.max_len), p.capacity)) return;
   float sum = 0.f;
   for (int c = 0; c < p.num_chunks; ++c)
@@ -294,8 +552,19 @@ cudaError_t launch_tw(const CUtensorMap& tq, const CUtensorMap& tk, const TokenW
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_done[dev] = true;
   }
-  kern<<<dim3(p.h_k * p.num_chunks, (p.max_len + 127) / 128, p.b), kTwThreads, smem, stream>>>(tq, tk, p);
-  return cudaGetLastError();
+  const int64_t items = static_cast<int64_t>((p.max_len + p.item_keys - 1) / p.item_keys) * p.h_k * p.num_chunks * p.b;
+  const int64_t slots = 148 * (HD > 128 ? 1 : 2);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(items < slots ? items : slots));
+  cfg.blockDim = dim3(kTwThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.dependent_launch ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, tq, tk, p);
 }
 
 }  // namespace
@@ -315,6 +584,8 @@ cudaError_t launch_weights_finish(const WeightsFinishParams& p, cudaStream_t str
   return cudaLaunchKernelEx(&cfg, weights_finish_kernel, p);
 }
 
+int token_weights_item_keys(int d) { return 128 * tw_halves(d); }
+
 cudaError_t launch_token_weights(int dtype, const CUtensorMap& tq, const CUtensorMap& tk, const TokenWeightsParams& p,
                                  cudaStream_t stream) {
   const bool bf = dtype == FA_B200_BF16;
@@ -328,8 +599,16 @@ cudaError_t launch_token_weights(int dtype, const CUtensorMap& tq, const CUtenso
   if (e != cudaSuccess || p.num_chunks == 1) return e;
   const int most = p.max_len < p.capacity ? p.max_len : p.capacity;
   if (most <= 0) return cudaSuccess;
-  token_weights_join_kernel<<<dim3((most + 255) / 256, p.h_k, p.b), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((most + 255) / 256, p.h_k, p.b);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.dependent_launch ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, token_weights_join_kernel, p);
 }
 
 }  // namespace fa
