@@ -1298,7 +1298,7 @@ int fa_b200_kv_evict(const fa_b200_kv_evict_params* p, void* stream) {
       static_cast<int64_t>(p->sink_tokens) + p->recent_tokens > p->budget)
     return FA_B200_ERR_SHAPE;
   if (!budget_page_ok(p->page_size)) return FA_B200_ERR_PAGE;
-  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > (1ll << 30) || p->budget > (1 << 30)) return FA_B200_ERR_TOO_LARGE;
+  if (static_cast<int64_t>(p->max_blocks_per_seq) * p->page_size > (1ll << 30) || p->budget > 65535 * 64) return FA_B200_ERR_TOO_LARGE;
   if (p->b == 0) return FA_B200_OK;
   if (!p->k_cache || !p->v_cache || !p->block_table || !p->cache_seqlens || !p->weights_in || !p->weights_out || !p->kept_index ||
       !p->seqlens_out)

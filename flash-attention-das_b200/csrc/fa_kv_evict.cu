@@ -12,8 +12,8 @@ namespace fa {
 namespace {
 
 constexpr int kPickThreads = 1024;
-constexpr int kMoveThreads = 256;
-constexpr int kMoveUnroll = 8;     // 16-byte vectors in flight per thread
+constexpr int kMoveThreads = 256, kMoveMaxThreads = 1024;   // into new pages; in place, where one CTA does all
+constexpr int kMoveVectors = 8;    // 16-byte vectors in flight per thread
 
 __device__ __forceinline__ int evict_len(const KvEvictParams& p, int bi, bool report) {
   int len = max(p.seqlens[bi], 0);
@@ -90,12 +90,16 @@ __global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const KvEvictP
   for (int i = kept + tid; i < p.budget; i += kPickThreads) out[i] = -1;
 }
 
-// blockIdx: x piece (one CTA walks all pieces in place), y kv head and K / V, z sequence.
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const KvEvictParams p) {
-  const int hk = blockIdx.y >> 1, bi = blockIdx.z, tid = threadIdx.x;
+// A warp moves kMoveVectors * 32 / (16-byte vectors of a row) rows at a time: a lane looks up where one of them comes from
+// and goes to, then all lanes load kMoveVectors vectors each, rows side by side, and store them.
+// blockIdx: x kv head and K / V (fastest: the heads of a token lie side by side, and their kept positions are near each
+// other), y piece of the kept rows (one CTA walks all pieces in place), z sequence.
+// 32 sequences, 16384 tokens cut to 4096, 8 kv heads, bf16: 0.95 GB.
+__global__ void __launch_bounds__(kMoveMaxThreads) evict_move_kernel(const KvEvictParams p) {
+  const int hk = blockIdx.x >> 1, bi = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_wait();
   griddep_launch_dependents();
-  const bool is_v = blockIdx.y & 1;
+  const bool is_v = blockIdx.x & 1;
   const int len = evict_len(p, bi, false);
   const int kept = min(len, p.budget);
   const bool in_place = p.new_block_table == nullptr;
@@ -106,35 +110,39 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const KvEvictP
   const int dst_max = in_place ? p.max_blocks : p.new_max_blocks;
   uint8_t* pool = static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + hk * (is_v ? p.v_h : p.k_h);
   const int64_t blk = is_v ? p.v_blk : p.k_blk, row = is_v ? p.v_row : p.k_row;
-  const int nv = p.row_bytes >> 4;                                   // 16-byte vectors of a row
-  const int rows_per_pass = kMoveThreads / nv;                       // rows read side by side
-  const int piece = rows_per_pass * kMoveUnroll;
-  const int r_in = tid / nv, vec = tid - r_in * nv;
-  const bool live = r_in < rows_per_pass;
-  for (int first = blockIdx.x * piece; first < kept; first += gridDim.x * piece) {
-    uint4 v[kMoveUnroll];
-    uint8_t* dst[kMoveUnroll];
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int i = first + u * rows_per_pass + r_in;
-      dst[u] = nullptr;
-      if (!live || i >= kept) continue;
-      const int from = index[i];
-      if (in_place && from == i) continue;   // already there
-      const int sp = src_bt[from / p.page_size];
-      const int ds = i / p.page_size;
-      const int dp = ds < dst_max ? dst_bt[ds] : -1;
-      if (sp < 0 || sp >= p.num_blocks || dp < 0 || dp >= p.num_blocks) {
-        atomicOr(p.status, kRangeBit);
-        continue;
+  const int nv = p.row_bytes >> 4;                                   // 16-byte vectors of a row: 8, 16, 24 or 32
+  const int side = 32 / nv;                                          // rows side by side
+  const int rows = side * kMoveVectors;                              // of a warp at a time, at most 32
+  const int r_in = lane / nv, vec = lane - r_in * nv;
+  const int piece = rows * (blockDim.x >> 5);
+  for (int first = blockIdx.y * piece; first < kept; first += gridDim.y * piece) {
+    int64_t from = -1, to = -1;
+    const int i = first + warp * rows + lane;
+    if (lane < rows && i < kept) {
+      const int at = len <= p.budget ? i : index[i];
+      if (!(in_place && at == i)) {   // else it is there already
+        const int sp = src_bt[at / p.page_size], ds = i / p.page_size;
+        const int dp = ds < dst_max ? dst_bt[ds] : -1;
+        if (sp < 0 || sp >= p.num_blocks || dp < 0 || dp >= p.num_blocks) {
+          atomicOr(p.status, kRangeBit);
+        } else {
+          from = sp * blk + (at % p.page_size) * row;
+          to = dp * blk + (i % p.page_size) * row;
+        }
       }
-      v[u] = *reinterpret_cast<const uint4*>(pool + sp * blk + (from % p.page_size) * row + vec * 16);
-      dst[u] = pool + dp * blk + (i % p.page_size) * row + vec * 16;
+    }
+    uint4 v[kMoveVectors];
+#pragma unroll
+    for (int u = 0; u < kMoveVectors; ++u) {
+      const int64_t s = __shfl_sync(0xffffffffu, from, (u * side + r_in) & 31);
+      if (s >= 0 && r_in < side) v[u] = *reinterpret_cast<const uint4*>(pool + s + vec * 16);
     }
     if (in_place) __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u)
-      if (dst[u]) *reinterpret_cast<uint4*>(dst[u]) = v[u];
+    for (int u = 0; u < kMoveVectors; ++u) {
+      const int64_t d = __shfl_sync(0xffffffffu, to, (u * side + r_in) & 31);
+      if (d >= 0 && r_in < side) *reinterpret_cast<uint4*>(pool + d + vec * 16) = v[u];
+    }
   }
 }
 
@@ -152,13 +160,15 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t stream) {
   cfg.numAttrs = p.dependent_launch ? 1 : 0;
   const int64_t most = min(static_cast<int64_t>(p.max_blocks) * p.page_size, static_cast<int64_t>(p.capacity));
   cudaError_t e = most <= 4 * kPickThreads    ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<4, true>, p)
+                  : most <= 8 * kPickThreads  ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<8, true>, p)
                   : most <= 16 * kPickThreads ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<16, true>, p)
                                               : cudaLaunchKernelEx(&cfg, evict_pick_kernel<8, false>, p);
   if (e != cudaSuccess) return e;
-  const int piece = kMoveThreads / (p.row_bytes >> 4) * kMoveUnroll;
-  const int pieces = p.new_block_table ? (p.budget + piece - 1) / piece : 1;
-  cfg.gridDim = dim3(pieces, p.h_k * 2, p.b);
-  cfg.blockDim = dim3(kMoveThreads);
+  const bool in_place = p.new_block_table == nullptr;
+  const int threads = in_place ? kMoveMaxThreads : kMoveThreads;
+  const int piece = 32 / (p.row_bytes >> 4) * kMoveVectors * (threads / 32);
+  cfg.gridDim = dim3(p.h_k * 2, in_place ? 1 : (p.budget + piece - 1) / piece, p.b);
+  cfg.blockDim = dim3(threads);
   return cudaLaunchKernelEx(&cfg, evict_move_kernel, p);
 }
 
