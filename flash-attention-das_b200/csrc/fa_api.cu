@@ -235,7 +235,8 @@ struct DecodePlan {
   bool split;
 };
 
-DecodePlan plan_decode(const fa_b200_decode_params* p) {
+// `budget`: a call of fa_b200_decode_budget, whose caches are short or read in part.
+DecodePlan plan_decode(const fa_b200_decode_params* p, bool budget = false) {
   DecodePlan pl{};
   pl.status = FA_B200_OK;
   if (!p) { pl.status = FA_B200_ERR_NULL; return pl; }
@@ -296,6 +297,15 @@ DecodePlan plan_decode(const fa_b200_decode_params* p) {
         if (ctas_half > 296 || ctas_half * 4 < 296 * 3) break;
         part *= 2;
       }
+    }
+    // Budget calls whose grid would stay within two rounds of the 296 CTA slots: the shortest partitions that fit one round,
+    // down to four tiles, joined by the combine launch.  One sequence of 4099 tokens, 8 kv heads, bf16 (token weights): 25 us
+    // with 512 tokens merged in the kernel, 17.3 / 14.4 / 14.8 with 512 / 256 / 128 and the combine launch; 4 sequences of 4096
+    // listed tokens, fp16: 20.8 us merged in the kernel, 20.1 / 15.8 / 19.7 / 27.5 with 1024 / 512 / 256 / 128.
+    if (budget && rows * ((max_len + part - 1) / part) <= 2 * 296) {
+      int small = 4 * pl.tile;
+      while (small < max_len && rows * ((max_len + small - 1) / small) > 296) small *= 2;
+      if (small < part) part = small;
     }
     while (static_cast<int64_t>(part) * 256 < max_len) part *= 2;   // at most 256 partitions per sequence
     if (part < unit) part = unit;
@@ -644,7 +654,7 @@ static size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // e: page lists per kv head and / or token weights (fa_b200_decode_budget); nullptr: plain decode.
 static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_budget_params* e_, cudaStream_t stream) {
-  DecodePlan pl = plan_decode(p);
+  DecodePlan pl = plan_decode(p, e_ != nullptr);
   if (pl.status != FA_B200_OK) return pl.status;
   const bool per_head = e_ && e_->per_kv_head;
   const bool weights = e_ && e_->weights_out;
@@ -770,7 +780,7 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
     // with the merge in the kernel against 0.389 ms with the combine launch; bf16 CTAs are longer and HBM-bound, and
     // measured the same both ways.
     const int64_t ctas = static_cast<int64_t>(pl.num_partitions) * p->h_k * p->b;
-    const bool want = g_env.decode_merge == 2 || (g_env.decode_merge == 0 && ctas <= 2 * 296);
+    const bool want = !e_ && (g_env.decode_merge == 2 || (g_env.decode_merge == 0 && ctas <= 2 * 296));
     if (pl.num_partitions <= 256 && want) k.tickets = p->tickets ? p->tickets : stream_tickets(stream, static_cast<int64_t>(p->b) * p->h_k);
     merge_in_kernel = k.tickets != nullptr;
     if (merge_in_kernel) final_rows_to_caller();
@@ -791,8 +801,9 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
   if (e != cudaSuccess) return cuda_fail("decode launch", e);
   if (p->profile_stop_event) cudaEventRecord(static_cast<cudaEvent_t>(p->profile_stop_event), stream);
   g_launches++;
-  if (pl.split && !merge_in_kernel) {
-    CombineKernelParams c{};
+  CombineKernelParams c{};
+  const bool combine = pl.split && !merge_in_kernel;
+  if (combine) {
     c.dependent_launch = g_env.dependent_launch;
     c.o_partial = k.o_partial;
     c.lse_partial = k.lse_partial;
@@ -829,15 +840,20 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
       c.s_aux = p->s_aux;   // partials handed to the caller stay without the sink: its final combine adds it
       c.s_aux_dtype = p->s_aux_dtype;
     }
-    e = launch_combine(c, stream);
-    if (e != cudaSuccess) return cuda_fail("combine launch", e);
-    g_launches++;
   }
   if (weights) {
     WeightsFinishParams w{};
     w.scores = k.scores;
     w.score_stride = k.score_stride;
     w.lse = p->softmax_lse;
+    if (combine) {
+      w.lse_partial = k.lse_partial;
+      w.lse_part_stride = c.lse_part_stride;
+      w.num_parts = pl.num_partitions;
+      w.partition_tokens = pl.partition_tokens;
+      w.s_aux = p->s_aux;
+      w.s_aux_dtype = p->s_aux_dtype;
+    }
     w.seqlens = p->cache_seqlens;
     w.w_in = e_->weights_in;
     w.w_out = e_->weights_out;
@@ -850,8 +866,12 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
     w.window_left = k.window_left;
     w.decay = e_->decay;
     w.dependent_launch = g_env.dependent_launch;
-    e = launch_weights_finish(w, stream);
-    if (e != cudaSuccess) return cuda_fail("token weights launch", e);
+    e = launch_combine_weights(combine ? &c : nullptr, w, stream);
+    if (e != cudaSuccess) return cuda_fail("combine and token weights launch", e);
+    g_launches++;
+  } else if (combine) {
+    e = launch_combine(c, stream);
+    if (e != cudaSuccess) return cuda_fail("combine launch", e);
     g_launches++;
   }
   return FA_B200_OK;
@@ -869,7 +889,7 @@ int fa_b200_decode_budget(const fa_b200_decode_params* p, const fa_b200_decode_b
 
 size_t fa_b200_decode_budget_workspace_bytes(const fa_b200_decode_params* p, const fa_b200_decode_budget_params* e) {
   if (!e || e->struct_size != sizeof(fa_b200_decode_budget_params)) return 0;
-  DecodePlan pl = plan_decode(p);
+  DecodePlan pl = plan_decode(p, true);
   if (pl.status != FA_B200_OK) return 0;
   const size_t parts = decode_ws_bytes(p, pl);
   return e->weights_out ? align256(parts) + score_ws_bytes(p, pl) : parts;

@@ -7,6 +7,7 @@
 // its LSE-writing variant (csrc/flash_attn_hipc/src/flash_fwd_reduce.h:313-464).
 #include "fa_common.cuh"
 #include "fa_kernels.h"
+#include "fa_weights_finish.cuh"
 
 namespace fa {
 namespace {
@@ -18,14 +19,10 @@ constexpr int kCombineWarps = 4;
 // so a row with hundreds of partitions (one very long sequence) is not walked by a single warp.
 // NV: groups of 128 columns (ceil(d / 128)).
 template <int NV>
-__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const CombineKernelParams p) {
+__device__ __forceinline__ void combine_row(const CombineKernelParams& p, const int row) {
   __shared__ float red_max[kCombineWarps], red_sum[kCombineWarps];
   __shared__ float4 red_acc[kCombineWarps][NV][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x;
-  // launched with programmatic stream serialisation: the partials come from the kernel before this one
-  griddep_wait();
-  griddep_launch_dependents();
   const int sq = p.sq > 0 ? p.sq : 1;
   const int bi = row / (p.h * sq), hi = (row / sq) % p.h, ti = row % sq;
   int nparts = p.num_parts;
@@ -144,7 +141,52 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const Combi
   if (p.lse && lane == 0) p.lse[row] = empty ? (p.lse_empty_is_neg ? -INFINITY : INFINITY) : lse_tot;
 }
 
+template <int NV>
+__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const CombineKernelParams p) {
+  // launched with programmatic stream serialisation: the partials come from the kernel before this one
+  griddep_wait();
+  griddep_launch_dependents();
+  combine_row<NV>(p, blockIdx.x);
+}
+
+// The combine of a split decode that accumulates token weights, and the weights beside it (both need no more than the
+// decode kernel's partials): CTAs 0 .. rows - 1 combine, the others take kFinishTokens tokens of a (sequence, kv head) each.
+template <int NV>
+__global__ void __launch_bounds__(kCombineWarps * 32) combine_weights_kernel(const CombineKernelParams p, const WeightsFinishParams w) {
+  static_assert(kCombineWarps * 32 == kFinishThreads, "one block size");
+  __shared__ float sm_lse[16];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int rows = NV > 0 ? p.rows : 0;
+  if (NV > 0 && static_cast<int>(blockIdx.x) < rows) {
+    combine_row<NV == 0 ? 1 : NV>(p, blockIdx.x);
+    return;
+  }
+  const int i = blockIdx.x - rows, chunk = i % w.chunks, pair = i / w.chunks;
+  finish_tokens(w, chunk, pair % w.h_k, pair / w.h_k, sm_lse);
+}
+
 }  // namespace
+
+cudaError_t launch_combine_weights(const CombineKernelParams* c, const WeightsFinishParams& w_, cudaStream_t stream) {
+  WeightsFinishParams w = w_;
+  const int most = w.max_len < w.capacity ? w.max_len : w.capacity;
+  w.chunks = (most + kFinishTokens - 1) / kFinishTokens;
+  const int64_t grid = (c ? c->rows : 0) + static_cast<int64_t>(w.chunks) * w.h_k * w.b;
+  if (grid == 0) return cudaSuccess;
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kFinishThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = w.dependent_launch ? 1 : 0;
+  if (!c) return cudaLaunchKernelEx(&cfg, combine_weights_kernel<0>, CombineKernelParams{}, w);
+  return c->d > 128 ? cudaLaunchKernelEx(&cfg, combine_weights_kernel<2>, *c, w) : cudaLaunchKernelEx(&cfg, combine_weights_kernel<1>, *c, w);
+}
 
 cudaError_t launch_combine(const CombineKernelParams& p, cudaStream_t stream) {
   if (p.rows <= 0) return cudaSuccess;

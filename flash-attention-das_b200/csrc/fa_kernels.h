@@ -50,7 +50,7 @@ struct DecodeKernelParams {
   int* tickets;
   int32_t merge_lse_empty_is_neg;   // merged rows without keys: LSE -inf (partial convention) instead of +inf
   int32_t merge_sink;               // the merge adds the sink (s_aux) to the row sums
-  float* scores;                    // [b][h_k][sq * group][score_stride] fp32, log2 units, or nullptr: see launch_token_weights_finish
+  float* scores;                    // [b][h_k][sq * group][score_stride] fp32, log2 units, or nullptr: see launch_combine_weights
   int64_t score_stride;
   int32_t dependent_launch;         // launch with programmatic stream serialisation (the kernel waits by itself)
   int32_t test_withhold;            // FA_B200_TEST_HOOKS builds only: CTA (0, 0, 0) announces its first tile and never loads it
@@ -260,12 +260,17 @@ struct PageSelectParams {
 size_t page_select_workspace_bytes(int b, int h_k, int max_blocks);
 cudaError_t launch_page_select(int dtype, const PageSelectParams& p, cudaStream_t stream);
 
-// weights_out = decay * weights_in + sum over the rows of 2^(score - lse): second pass of a decode that wrote its
-// scores (DecodeKernelParams::scores) and its merged lse.
+// weights_out = decay * weights_in + sum over the rows of 2^(score - lse): second pass of a decode that wrote its scores
+// (DecodeKernelParams::scores), in the launch that combines its partials (c; nullptr: the decode was not split).
 struct WeightsFinishParams {
   const float* scores;
   int64_t score_stride;
-  const float* lse;          // (b, h, sq), natural log
+  const float* lse;          // (b, h, sq), natural log: the final one of a decode that was not split
+  const float* lse_partial;  // [num_parts][b][h][sq], partitions lse_part_stride apart, or nullptr
+  int64_t lse_part_stride;
+  int32_t num_parts, partition_tokens;
+  const void* s_aux;
+  int32_t s_aux_dtype;
   const int32_t* seqlens;
   const float* w_in;
   float* w_out;
@@ -274,8 +279,9 @@ struct WeightsFinishParams {
   int32_t causal, window_left;
   float decay;
   int32_t dependent_launch;
+  int32_t chunks;            // set by launch_combine_weights
 };
-cudaError_t launch_weights_finish(const WeightsFinishParams& p, cudaStream_t stream);
+cudaError_t launch_combine_weights(const CombineKernelParams* c, const WeightsFinishParams& w, cudaStream_t stream);
 
 struct KvEvictParams {
   int* status;

@@ -1,8 +1,5 @@
-// The weight that every cached key receives: sums of softmax probabilities over query rows.
-//
-// After a decode call.  The decode kernel leaves its scaled scores (log2 units) behind, rows x tokens in fp32: 4 bytes
-// per (query head, key) against 2 * d * element size bytes of K and V per (kv head, key), small enough to stay in L2.  Once the row's
-// log-sum-exp is known this kernel reads them back: w[t] = decay w[t] + sum_r 2^(s_rt - lse_r), rows in a fixed order.
+// The weight that every cached key receives: sums of softmax probabilities over query rows.  After a decode call:
+// fa_weights_finish.cuh.
 //
 // Of a prompt.  Given every query's log-sum-exp the weight of key t is a plain sum over the queries, with no running
 // maximum: a CTA takes 128 keys of one kv head (256 above d = 128) as the A operand and walks the query tiles that see them,
@@ -26,36 +23,6 @@
 
 namespace fa {
 namespace {
-
-constexpr int kFinishThreads = 256;
-
-__global__ void __launch_bounds__(kFinishThreads) weights_finish_kernel(const WeightsFinishParams p) {
-  __shared__ float sm_lse[16];
-  const int hk = blockIdx.y, bi = blockIdx.z;
-  const int rows = p.sq * p.group;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int len = min(min(p.seqlens[bi], p.max_len), p.capacity);
-  const int tok = blockIdx.x * kFinishThreads + threadIdx.x;
-  if (static_cast<int>(blockIdx.x) * kFinishThreads >= len) return;
-  if (threadIdx.x < rows) {   // row r is query token r / group, head r % group
-    const int r = threadIdx.x;
-    sm_lse[r] = p.lse[(static_cast<int64_t>(bi) * p.h + hk * p.group + r % p.group) * p.sq + r / p.group] * kLog2e;
-  }
-  __syncthreads();
-  if (tok >= len) return;
-  const float* s = p.scores + (static_cast<int64_t>(bi) * p.h_k + hk) * rows * p.score_stride + tok;
-  const int full = min(p.seqlens[bi], p.max_len);
-  float sum = 0.f;
-  for (int r = 0; r < rows; ++r) {
-    const int behind = p.sq - 1 - r / p.group;   // query tokens after this row's
-    const bool seen = !(p.causal && tok >= full - behind) &&
-                      !(p.window_left >= 0 && tok < full - behind - 1 - p.window_left);
-    if (seen) sum += exp2f(s[r * p.score_stride] - sm_lse[r]);
-  }
-  const float before = p.w_in ? p.w_in[bi * p.win_b + hk * p.win_h + tok] * p.decay : 0.f;
-  p.w_out[bi * p.wout_b + hk * p.wout_h + tok] = before + sum;
-}
 
 // 128-key halves of a CTA: two CTAs per SM with one up to d = 128, one CTA with two above (shared memory).  Eight warps take
 // the sums either way: with one half, two warps share 32 keys and take half of a tile's columns each (16 warps per SM keep the
@@ -568,21 +535,6 @@ cudaError_t launch_tw(const CUtensorMap& tq, const CUtensorMap& tk, const TokenW
 }
 
 }  // namespace
-
-cudaError_t launch_weights_finish(const WeightsFinishParams& p, cudaStream_t stream) {
-  const int most = p.max_len < p.capacity ? p.max_len : p.capacity;
-  if (most <= 0) return cudaSuccess;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((most + kFinishThreads - 1) / kFinishThreads, p.h_k, p.b);
-  cfg.blockDim = dim3(kFinishThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.dependent_launch ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, weights_finish_kernel, p);
-}
 
 int token_weights_item_keys(int d) { return 128 * tw_halves(d); }
 

@@ -1435,7 +1435,6 @@ def decode_budget(q, kcache, vcache, block_table, seqlens, softmax_scale, is_cau
         ws = _workspace(dev, int(_lib.fa_b200_decode_budget_workspace_bytes(ctypes.byref(p), ctypes.byref(e))))
         if ws is not None:
             p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-            _tickets = _own_tickets(p, dev, b * h_k)
         _check(_lib.fa_b200_decode_budget(ctypes.byref(p), ctypes.byref(e), _stream(q)), "decode_budget")
     return out, lse, w
 

@@ -206,8 +206,10 @@ def test_sparse_attention(fa, monkeypatch, qt, kv, d, h, h_k, sq, page, k, parti
     assert cuda.device_status() == 0
 
 
-def test_sparse_attention_over_all_pages_is_the_dense_call(fa):
+def test_sparse_attention_over_all_pages_is_the_dense_call(fa, monkeypatch):
+    """Bit for bit, where neither is split (they split by rules of their own)."""
     m, _ = fa
+    monkeypatch.setenv("FA_B200_DECODE_PARTITION", "2048")
     g = gen(6)
     lens = [1500, 64, 0, 777]
     kc, vc, bt, sl, kd, vd = pools(g, lens, 2, 64, BF)
@@ -268,8 +270,10 @@ def test_decode_with_weights(fa, monkeypatch, qt, kv, d, h, h_k, sq, page, parti
                 r = w[i, x, :n].double() * decay + rw[i][x]
                 # each probability is off by at most 2 tol of itself (score and log-sum-exp), the sum by a rounding more
                 assert ((got[i, x, :n].double() - r).abs() <= (2 * tol + 2.0 ** -20) * r.abs()).all(), (i, x)
-    # the attention itself is the call without weights, bit for bit
+    # the attention itself is the call without weights, bit for bit where neither is split
     if not sink and window < 0:
+        monkeypatch.setenv("FA_B200_DECODE_PARTITION", "2048")
+        out, _ = m.flash_attn_with_kvcache_weights(*args, w.cuda(), causal=True, **kw)
         plain = m.flash_attn_with_kvcache(q.cuda(), kd, vd, cache_seqlens=sl.cuda(), block_table=bt.cuda(), causal=True, **kw)
         assert torch.equal(plain, out)
     assert cuda.device_status() == 0
