@@ -32,6 +32,28 @@ std::atomic<int> g_test_withhold{0};   // the next decode / two-tile prefill lau
 thread_local char g_last_error[256] = "";
 thread_local char g_launch_info[320] = "";
 
+// What the calling thread's last decode call did.
+struct DecodeInfo {
+  int dtype, kv_e4m3, kv_e5m2, d, b, h, h_k, sq, page_size, partition_tokens, num_partitions;
+  bool split, merge_in_kernel;
+};
+thread_local DecodeInfo g_decode_info;
+thread_local bool g_info_pending = false;   // g_launch_info is to be made from g_decode_info
+const char* launch_info() {
+  if (g_info_pending) {
+    const DecodeInfo& i = g_decode_info;
+    const char* dt = i.dtype == FA_B200_E4M3 ? "e4m3" : (i.dtype == FA_B200_BF16 ? "bf16" : "f16");
+    const char* cache = i.kv_e4m3 ? (i.kv_e5m2 ? "+e5m2 cache" : "+e4m3 cache") : "";
+    snprintf(g_launch_info, sizeof(g_launch_info),
+             "fa_b200 decode: kernel=decode_paged dtype=%s%s d=%d b=%d h=%d h_k=%d seqlen_q=%d page=%d partition_tokens=%d "
+             "partitions=%d grid=(%d,%d,%d) threads=160 merge=%s",
+             dt, cache, i.d, i.b, i.h, i.h_k, i.sq, i.page_size, i.partition_tokens, i.num_partitions, i.num_partitions, i.h_k, i.b,
+             !i.split ? "none (one partition)" : (i.merge_in_kernel ? "in-kernel (last CTA per sequence and kv head)" : "combine kernel"));
+    g_info_pending = false;
+  }
+  return g_launch_info;
+}
+
 void set_error(const char* what, const char* detail) {
   snprintf(g_last_error, sizeof(g_last_error), "%s: %s", what, detail ? detail : "");
 }
@@ -340,7 +362,7 @@ __attribute__((visibility("default"))) void fa_b200_test_withhold_load(int on) {
 
 int fa_b200_abi_version(void) { return FA_B200_ABI_VERSION; }
 void fa_b200_set_print_param(int on) { g_print_param.store(on < 0 ? -1 : (on ? 1 : 0)); }
-const char* fa_b200_last_launch_info(void) { return g_launch_info; }
+const char* fa_b200_last_launch_info(void) { return launch_info(); }
 uint64_t fa_b200_launch_count(void) { return g_launches.load(); }
 const char* fa_b200_last_cuda_error(void) { return g_last_error; }
 
@@ -785,17 +807,10 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
     merge_in_kernel = k.tickets != nullptr;
     if (merge_in_kernel) final_rows_to_caller();
   }
-  {
-    const char* dt = p->dtype == FA_B200_E4M3 ? "e4m3" : (p->dtype == FA_B200_BF16 ? "bf16" : "f16");
-    const char* cache = p->kv_e4m3 ? (p->kv_e5m2 ? "+e5m2 cache" : "+e4m3 cache") : "";
-    snprintf(g_launch_info, sizeof(g_launch_info),
-             "fa_b200 decode: kernel=decode_paged dtype=%s%s d=%d b=%d h=%d h_k=%d seqlen_q=%d page=%d partition_tokens=%d "
-             "partitions=%d grid=(%d,%d,%d) threads=160 merge=%s",
-             dt, cache, p->d, p->b, p->h, p->h_k, k.sq, p->page_size, pl.partition_tokens, pl.num_partitions,
-             pl.num_partitions, p->h_k, p->b,
-             !pl.split ? "none (one partition)" : (merge_in_kernel ? "in-kernel (last CTA per sequence and kv head)" : "combine kernel"));
-    if (print_param()) fprintf(stderr, "%s\n", g_launch_info);
-  }
+  g_decode_info = DecodeInfo{p->dtype, p->kv_e4m3, p->kv_e5m2, p->d, p->b, p->h, p->h_k, k.sq, p->page_size, pl.partition_tokens,
+                             pl.num_partitions, pl.split, merge_in_kernel};
+  g_info_pending = true;   // put into words when somebody asks: formatting is a good part of a microsecond per call
+  if (print_param()) fprintf(stderr, "%s\n", launch_info());
   if (p->profile_start_event) cudaEventRecord(static_cast<cudaEvent_t>(p->profile_start_event), stream);
   cudaError_t e = launch_decode(p->dtype, tk, tv, k, stream);
   if (e != cudaSuccess) return cuda_fail("decode launch", e);
@@ -1105,6 +1120,7 @@ static int fwd_common(const fa_b200_fwd_params* p, void* stream_, bool sparse) {
                                          "prefill_pair (persistent, two heads of a GQA group per item)",
                                          "prefill_dense (persistent, double-buffered scores)"};
     const char* dt = p->dtype == FA_B200_E4M3 ? "e4m3" : (p->dtype == FA_B200_BF16 ? "bf16" : "f16");
+    g_info_pending = false;
     snprintf(g_launch_info, sizeof(g_launch_info),
              "fa_b200 prefill: kernel=%s dtype=%s d=%d d_v=%d b=%d h=%d h_k=%d seqlen_q=%d seqlen_k=%d varlen=%d paged=%d "
              "tile_lists=%d causal=%d window=(%d,%d) q_blocks=%d",
