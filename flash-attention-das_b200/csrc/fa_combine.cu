@@ -171,7 +171,12 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_weights_kernel(con
 cudaError_t launch_combine_weights(const CombineKernelParams* c, const WeightsFinishParams& w_, cudaStream_t stream) {
   WeightsFinishParams w = w_;
   const int most = w.max_len < w.capacity ? w.max_len : w.capacity;
-  w.chunks = (most + kFinishTokens - 1) / kFinishTokens;
+  // Chunks of a CTA: one while that leaves room on the GPU (16 CTAs on each of 148 SMs), up to eight, which share a CTA's
+  // look at the lengths and partial log-sum-exps.
+  const int chunks = (most + kFinishTokens - 1) / kFinishTokens;
+  w.loops = 1;
+  while (w.loops < 8 && static_cast<int64_t>(chunks) * w.h_k * w.b / (2 * w.loops) >= 148 * 8) w.loops *= 2;
+  w.chunks = (chunks + w.loops - 1) / w.loops;
   const int64_t grid = (c ? c->rows : 0) + static_cast<int64_t>(w.chunks) * w.h_k * w.b;
   if (grid == 0) return cudaSuccess;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;

@@ -279,7 +279,7 @@ struct WeightsFinishParams {
   int32_t causal, window_left;
   float decay;
   int32_t dependent_launch;
-  int32_t chunks;            // set by launch_combine_weights
+  int32_t chunks, loops;     // set by launch_combine_weights: CTAs per (sequence, kv head), and their chunks of tokens
 };
 cudaError_t launch_combine_weights(const CombineKernelParams* c, const WeightsFinishParams& w, cudaStream_t stream);
 

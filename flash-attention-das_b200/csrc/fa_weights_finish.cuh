@@ -50,49 +50,57 @@ __device__ __forceinline__ void finish_lse(const WeightsFinishParams& p, int bi,
   }
 }
 
-// Tokens chunk * kFinishTokens .. of one (sequence, kv head).  sm_lse: 16 floats of shared memory.
-__device__ __forceinline__ void finish_tokens(const WeightsFinishParams& p, int chunk, int hk, int bi, float* sm_lse) {
+// Chunks first * loops .. of kFinishTokens tokens of one (sequence, kv head).  sm_lse: 16 floats of shared memory.
+__device__ __forceinline__ void finish_tokens(const WeightsFinishParams& p, int first, int hk, int bi, float* sm_lse) {
   const int rows = p.sq * p.group;
   const int full = min(p.seqlens[bi], p.max_len), len = min(full, p.capacity);
-  if (chunk * kFinishTokens >= len) return;
-  const int tok = chunk * kFinishTokens + 4 * threadIdx.x;
-  const float* in = p.w_in ? p.w_in + bi * p.win_b + hk * p.win_h + tok : nullptr;
-  float* out = p.w_out + bi * p.wout_b + hk * p.wout_h + tok;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
-  if (in && tok < len) {   // on its way while the rows' log-sum-exps are looked up
-    if (tok + 4 <= len && (reinterpret_cast<uintptr_t>(in) & 15) == 0) {
-      const float4 v = *reinterpret_cast<const float4*>(in);
-      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  int tok = first * p.loops * kFinishTokens;
+  if (tok >= len) return;
+  tok += 4 * threadIdx.x;
+  const float* in = p.w_in ? p.w_in + bi * p.win_b + hk * p.win_h : nullptr;
+  float* out = p.w_out + bi * p.wout_b + hk * p.wout_h;
+  const float* s = p.scores + (static_cast<int64_t>(bi) * p.h_k + hk) * rows * p.score_stride;
+  const bool in16 = (reinterpret_cast<uintptr_t>(in) & 15) == 0, out16 = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const bool all = p.window_left < 0 && (p.sq == 1 || !p.causal);   // every row sees every key
+  bool first_pass = true;
+  for (int l = 0; l < p.loops; ++l, tok += kFinishTokens) {
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    if (in && tok < len) {   // on its way while the rows' log-sum-exps are looked up
+      if (tok + 4 <= len && in16) {
+        const float4 v = *reinterpret_cast<const float4*>(in + tok);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tok + e < len) w[e] = in[tok + e];
+      }
+    }
+    if (first_pass) {
+      finish_lse(p, bi, hk, full, sm_lse);
+      __syncthreads();
+      first_pass = false;
+    }
+    if (tok >= len) return;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(s + r * p.score_stride + tok);   // rows are padded to whole tiles
+      const float lse = sm_lse[r];
+      const float x[4] = {exp2f(v.x - lse), exp2f(v.y - lse), exp2f(v.z - lse), exp2f(v.w - lse)};
+      const int behind = p.sq - 1 - r / p.group;   // query tokens after this row's
+      const int hi = p.causal ? full - behind : full, lo = p.window_left >= 0 ? full - behind - 1 - p.window_left : 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += (all || (tok + e < hi && tok + e >= lo)) ? x[e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = w[e] * p.decay + sum[e];
+    if (tok + 4 <= len && out16) {
+      *reinterpret_cast<float4*>(out + tok) = make_float4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (tok + e < len) w[e] = in[e];
+        if (tok + e < len) out[tok + e] = w[e];
     }
-  }
-  finish_lse(p, bi, hk, full, sm_lse);
-  __syncthreads();
-  if (tok >= len) return;
-  const float* s = p.scores + (static_cast<int64_t>(bi) * p.h_k + hk) * rows * p.score_stride + tok;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const bool all = p.window_left < 0 && (p.sq == 1 || !p.causal);   // every row sees every key
-#pragma unroll 4
-  for (int r = 0; r < rows; ++r) {
-    const float4 v = *reinterpret_cast<const float4*>(s + r * p.score_stride);   // rows are padded to whole tiles
-    const float l = sm_lse[r];
-    const float x[4] = {exp2f(v.x - l), exp2f(v.y - l), exp2f(v.z - l), exp2f(v.w - l)};
-    const int behind = p.sq - 1 - r / p.group;   // query tokens after this row's
-    const int hi = p.causal ? full - behind : full, lo = p.window_left >= 0 ? full - behind - 1 - p.window_left : 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += (all || (tok + e < hi && tok + e >= lo)) ? x[e] : 0.f;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = w[e] * p.decay + sum[e];
-  if (tok + 4 <= len && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-    *reinterpret_cast<float4*>(out) = make_float4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (tok + e < len) out[e] = w[e];
   }
 }
 

@@ -25,8 +25,6 @@ import torch
 
 import flash_attn_2_cuda as flash_attn_cuda
 
-from .flash_attn_interface import _no_backward, maybe_contiguous
-
 
 def kvcache_page_bounds(
     k_cache,
@@ -42,7 +40,6 @@ def kvcache_page_bounds(
     its pages), each from all of its rows below cache_seqlens; other pages keep what they have.  A page that sequences share
     has to be full in all of them.  ``page_bounds`` None: a new tensor, zero in the pages of no sequence, of ``dtype`` (default:
     the cache's type, bf16 for an fp8 cache)."""
-    _no_backward(k_cache)
     if new_tokens is not None and new_tokens <= 0:
         raise ValueError("new_tokens must be positive (None: every page)")
     if page_bounds is None:
@@ -52,7 +49,7 @@ def kvcache_page_bounds(
         page_bounds = torch.zeros((nb, h_k, 2, d), dtype=dtype, device=k_cache.device)
     elif dtype is not None and dtype != page_bounds.dtype:
         raise ValueError("dtype is the type of a new page_bounds: pass one or the other")
-    return flash_attn_cuda.page_bounds(k_cache, maybe_contiguous(block_table), cache_seqlens, page_bounds, new_tokens or 0)
+    return flash_attn_cuda.page_bounds(k_cache, block_table, cache_seqlens, page_bounds, new_tokens or 0)
 
 
 def kvcache_select_pages(
@@ -76,8 +73,7 @@ def kvcache_select_pages(
     Returns (page_table, seqlens, page_index): page_table int32 (batch, nheads_k, num_pages) the physical pages in the order of
     the sequence, -1 behind them; seqlens int32 (batch, nheads_k) the tokens in them; page_index their positions in the
     sequence.  The first two are what ``sparse_attn_with_kvcache`` takes.  A sequence of at most num_pages pages keeps all."""
-    _no_backward(q, page_bounds)
-    return flash_attn_cuda.page_select(maybe_contiguous(q), page_bounds, maybe_contiguous(block_table), cache_seqlens, page_size,
+    return flash_attn_cuda.page_select(q, page_bounds, block_table, cache_seqlens, page_size,
                                        num_pages, sink_pages, recent_pages)
 
 
@@ -102,14 +98,13 @@ def sparse_attn_with_kvcache(
     descales as there; with several query tokens and ``causal`` the last listed tokens are taken for the new ones, as
     ``kvcache_select_pages`` provides.  Returns out, or (out, softmax_lse (batch, nheads, seqlen_q)): the softmax is that of the
     listed pages; a head without tokens returns 0 and an lse of +inf."""
-    _no_backward(q, k_cache, v_cache)
-    q = maybe_contiguous(q)
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)
     if page_table.dim() != 3:
         raise RuntimeError("page_table must have shape (batch, nheads_k, n)")
-    out, lse, _ = flash_attn_cuda.decode_budget(q, k_cache, v_cache, maybe_contiguous(page_table), seqlens, softmax_scale, causal, out,
-                                                maybe_contiguous(s_aux), -1, None, None, 1.0, q_descale, k_descale, v_descale)
+    out, lse, _ = flash_attn_cuda.decode_budget(q, k_cache, v_cache, page_table, seqlens, softmax_scale, causal, out,
+                                                s_aux, -1, None, None, 1.0, q_descale, k_descale, v_descale,
+                                                return_softmax_lse)
     return (out, lse) if return_softmax_lse else out
 
 
@@ -142,8 +137,6 @@ def flash_attn_with_kvcache_weights(
     given: from zero.  Without ``token_weights_out`` it is updated in place.  Entries at and behind the length are left as they
     are.  seqlen_q x heads per kv head <= 16 (prompts: ``attn_token_weights``).  A sink (s_aux) takes part in the softmax
     and in no key's weight.  Returns (out, token_weights_out), or (out, softmax_lse, token_weights_out)."""
-    _no_backward(q, k_cache, v_cache)
-    q = maybe_contiguous(q)
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)
     if block_table.dim() != 2:
@@ -152,8 +145,8 @@ def flash_attn_with_kvcache_weights(
         raise NotImplementedError("a right window bound with several decode tokens is outside the B200 hot path of this build")
     if token_weights is None and token_weights_out is None:
         raise RuntimeError("token_weights or token_weights_out is required")
-    out, lse, w = flash_attn_cuda.decode_budget(q, k_cache, v_cache, maybe_contiguous(block_table), cache_seqlens, softmax_scale, causal,
-                                                out, maybe_contiguous(s_aux), window_size[0], token_weights, token_weights_out,
+    out, lse, w = flash_attn_cuda.decode_budget(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, causal,
+                                                out, s_aux, window_size[0], token_weights, token_weights_out,
                                                 decay, q_descale, k_descale, v_descale)
     return (out, lse, w) if return_softmax_lse else (out, w)
 
@@ -183,11 +176,10 @@ def attn_token_weights(
     positions (causal: bottom-right aligned); softmax_lse fp32 (nheads, total_q): what flash_attn_varlen_func(...,
     return_softmax_lse=True) returned for them; k_cache: the paged keys, of q's type.  token_weights as in
     ``flash_attn_with_kvcache_weights``.  max_seqlen_q: an upper bound on the sequences' queries.  Returns token_weights_out."""
-    _no_backward(q, k_cache)
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)
-    return flash_attn_cuda.token_weights(maybe_contiguous(q), k_cache, softmax_lse, cu_seqlens_q, max_seqlen_q, cache_seqlens,
-                                         maybe_contiguous(block_table), token_weights, softmax_scale, causal, decay, token_weights_out)
+    return flash_attn_cuda.token_weights(q, k_cache, softmax_lse, cu_seqlens_q, max_seqlen_q, cache_seqlens,
+                                         block_table, token_weights, softmax_scale, causal, decay, token_weights_out)
 
 
 def kvcache_evict(
@@ -215,10 +207,9 @@ def kvcache_evict(
 
     Returns (kept_index, new_seqlens): kept_index int32 (batch, nheads_k, budget) the kept positions, ascending, -1 behind
     them; new_seqlens int32 (batch,) = min(cache_seqlens, budget)."""
-    _no_backward(k_cache, v_cache)
     if recent_tokens is None:
         recent_tokens = max(0, budget - sink_tokens) // 4
     if sink_tokens < 0 or recent_tokens < 0 or sink_tokens + recent_tokens > budget:
         raise ValueError("sink_tokens and recent_tokens must not be negative and have to fit the budget")
-    return flash_attn_cuda.kv_evict(k_cache, v_cache, maybe_contiguous(block_table), cache_seqlens, token_weights, budget, sink_tokens,
-                                    recent_tokens, maybe_contiguous(new_block_table), token_weights_out)
+    return flash_attn_cuda.kv_evict(k_cache, v_cache, block_table, cache_seqlens, token_weights, budget, sink_tokens,
+                                    recent_tokens, new_block_table, token_weights_out)

@@ -375,8 +375,12 @@ def last_launch_info() -> str:
 _KERNEL_CHOICE = {"single": 1, "pair": 2, "dense": 3}
 
 
+_environ = getattr(os.environ, "_data", None)      # the mapping behind os.environ: no encoding of the name per look
+_PARTITION = os.environ.encodekey("FA_B200_DECODE_PARTITION") if _environ is not None else None
+
+
 def _env_partition() -> int:
-    v = os.environ.get("FA_B200_DECODE_PARTITION")
+    v = os.environ.get("FA_B200_DECODE_PARTITION") if _environ is None else _environ.get(_PARTITION)
     return int(v) if v else 0
 
 
@@ -1326,8 +1330,9 @@ _decode_budget_bytes = _raw("fa_b200_decode_budget_workspace_bytes", _cc, _cc, r
 _token_weights_raw = _raw("fa_b200_token_weights", _cc, _c_vp)
 _token_weights_bytes = _raw("fa_b200_token_weights_workspace_bytes", _cc, restype=ctypes.c_size_t)
 _kv_evict_raw = _raw("fa_b200_kv_evict", _cc, _c_vp)
-_current_device = torch.cuda.current_device
-_capturing = torch.cuda.is_current_stream_capturing
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+_grad = torch.is_grad_enabled
 _ERR_WORKSPACE = 8
 
 
@@ -1357,6 +1362,11 @@ def _run_on(index, what, call, size):
     finally:
         if before != index:
             torch.cuda.set_device(before)
+
+
+def _forward_only(*tensors):
+    if any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("the B200 hot path is forward only: call under torch.no_grad() or detach inputs")
 
 
 def _check_tables(block_table, cache_seqlens, index, what):
@@ -1408,6 +1418,8 @@ def _weights_args(w_in, w_out, b, h_k, index, what):
 
 def page_bounds(k_cache, block_table, cache_seqlens, bounds, new_tokens=0):
     """fa_b200_page_bounds: writes ``bounds`` (num_blocks, h_k, 2, d), fp16 / bf16."""
+    if _grad():
+        _forward_only(k_cache)
     s, st, index = _check_cache(k_cache, "page_bounds")
     ts, t_stride = _check_tables(block_table, cache_seqlens, index, "page_bounds")
     nb, page, h_k, d = s
@@ -1423,7 +1435,12 @@ def page_bounds(k_cache, block_table, cache_seqlens, bounds, new_tokens=0):
 
 def page_select(q, bounds, block_table, cache_seqlens, page_size, num_pages, sink_pages=1, recent_pages=1):
     """fa_b200_page_select: (page_table, seqlens, page_index)."""
+    if _grad():
+        _forward_only(q, bounds)
     qs, qst, index = q.shape, q.stride(), q.get_device()
+    if qst[-1] != 1:
+        q = q.contiguous()
+        qst = q.stride()
     if not (index >= 0 and len(qs) == 4 and qst[3] == 1 and q.dtype in _HALF):
         _require(False, "page_select: q must be an fp16 / bf16 CUDA tensor (batch, seqlen_q, nheads, d) with contiguous last dimension")
     b, sq, h, d = qs
@@ -1458,12 +1475,19 @@ def _descale_args(name, t, b, h_k):
 
 def decode_budget(q, kcache, vcache, block_table, seqlens, softmax_scale, is_causal=False, out=None, s_aux=None,
                   window_left=-1, token_weights=None, token_weights_out=None, decay=1.0, q_descale=None, k_descale=None,
-                  v_descale=None):
+                  v_descale=None, need_lse=True):
     """fa_b200_decode_budget: decode over the pages of ``block_table`` (b, n), or (b, h_k, n) with ``seqlens`` (b, h_k), and,
     when token weights are given, the weight of every key.  Returns (out, softmax_lse, token weights or None)."""
-    _unsupported(_is_transposed_v(vcache), "a transposed V pool (layout 0)")
+    if _grad():
+        _forward_only(q, kcache, vcache)
+    vst = vcache.stride()
+    if len(vst) == 4 and vst[3] != 1 and vst[1] == 1:
+        _unsupported(True, "a transposed V pool (layout 0)")
     ks, kst, index = _check_cache(kcache, "decode_budget", vcache)
     qs, qst, qt, kt = q.shape, q.stride(), q.dtype, kcache.dtype
+    if qst[-1] != 1:
+        q = q.contiguous()
+        qst = q.stride()
     fp8_kv = qt in _HALF and kt in _FP8
     if not (len(qs) == 4 and qst[3] == 1 and q.get_device() == index):
         _require(False, "q must be a CUDA tensor (batch, seqlen_q, nheads, d) on the caches' device with contiguous last dimension")
@@ -1478,6 +1502,9 @@ def decode_budget(q, kcache, vcache, block_table, seqlens, softmax_scale, is_cau
     if fp8_kv and q_descale is not None:
         _unsupported(True, "an fp8 KV cache under 16-bit queries with q_descale")
     ts, tst, ls = block_table.shape, block_table.stride(), seqlens.shape
+    if tst[-1] != 1 and ts[-1] > 1:
+        block_table = block_table.contiguous()
+        tst = block_table.stride()
     per_head = len(ts) == 3
     if not (block_table.dtype is torch.int32 and block_table.get_device() == index and (tst[-1] == 1 or ts[-1] <= 1) and
             ts[:-1] == ((b, h_k) if per_head else (b,))):
@@ -1493,37 +1520,49 @@ def decode_budget(q, kcache, vcache, block_table, seqlens, softmax_scale, is_cau
     else:
         odt = _out_dtype(q, None)
         out = q.new_empty(qs, dtype=odt)
-    lse = q.new_empty((b, h, sq), dtype=torch.float32)
+    lse = q.new_empty((b, h, sq), dtype=torch.float32) if need_lse else None
     w = None
     if token_weights is not None or token_weights_out is not None:
         w, (wi, wo, wi_b, wi_h, wo_b, wo_h, capacity) = _weights_args(token_weights, token_weights_out, b, h_k, index, "token weights")
         e = _PACK_BUDGET.pack(_PACK_BUDGET.size, per_head, tst[1] if per_head else 0, wi, wo, wi_b, wi_h, wo_b, wo_h, capacity, decay)
     else:
         e = _PACK_BUDGET.pack(_PACK_BUDGET.size, per_head, tst[1] if per_head else 0, 0, 0, 0, 0, 0, 0, 0, 1.0)
-    qd = _descale_args("q_descale", q_descale, b, h_k)
-    kd = _descale_args("k_descale", k_descale, b, h_k)
-    vd = _descale_args("v_descale", v_descale, b, h_k)
+    qd = kd = vd = (0, 0, 0)
+    if q_descale is not None:
+        qd = _descale_args("q_descale", q_descale, b, h_k)
+    if k_descale is not None:
+        kd = _descale_args("k_descale", k_descale, b, h_k)
+    if v_descale is not None:
+        vd = _descale_args("v_descale", v_descale, b, h_k)
     sink, sink_dt = 0, 0
     if s_aux is not None:
+        s_aux = s_aux.contiguous()
         holder = DecodeParams()
         _set_sinks(holder, s_aux, h)
         sink, sink_dt = holder.s_aux, holder.s_aux_dtype
     ev0, ev1 = (0, 0) if _profile_events is None else (_profile_events[0].cuda_event, _profile_events[1].cuda_event)
-    ost, vst = out.stride(), vcache.stride()
-    head = (_PACK_DECODE.size, q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), lse.data_ptr(), qst[0], qst[2], ost[0],
-            ost[2], kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], block_table.data_ptr(), tst[0], seqlens.data_ptr(), b, h, h_k, d, nb, page,
-            ts[-1], softmax_scale, _DT[qt], _DT[odt], qd[0], kd[0], vd[0], qd[1], qd[2], kd[1], kd[2], vd[1], vd[2], _env_partition(), 0)
-    tail = (0, 0, ev0, ev1, sink, sink_dt, window_left >= 0, window_left, 0, sq, bool(is_causal), qst[1], ost[1], fp8_kv,
-            fp8_kv and kt is torch.float8_e5m2, 0)
-    pack = _PACK_DECODE.pack
-    _run_on(index, "decode_budget", lambda ws, n, stream: _decode_budget_raw(pack(*head, ws, n, *tail), e, stream),
-            lambda ws, n: _decode_budget_bytes(pack(*head, ws, n, *tail), e))
+    ost = out.stride()
+
+    def params(ws, n):
+        return _PACK_DECODE.pack(
+            _PACK_DECODE.size, q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), qst[0],
+            qst[2], ost[0], ost[2], kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], block_table.data_ptr(), tst[0], seqlens.data_ptr(), b, h, h_k,
+            d, nb, page, ts[-1], softmax_scale, _DT[qt], _DT[odt], qd[0], kd[0], vd[0], qd[1], qd[2], kd[1], kd[2], vd[1], vd[2],
+            _env_partition(), 0, ws, n, 0, 0, ev0, ev1, sink, sink_dt, window_left >= 0, window_left, 0, sq, bool(is_causal), qst[1], ost[1],
+            fp8_kv, fp8_kv and kt is torch.float8_e5m2, 0)
+
+    _run_on(index, "decode_budget", lambda ws, n, stream: _decode_budget_raw(params(ws, n), e, stream),
+            lambda ws, n: _decode_budget_bytes(params(ws, n), e))
     return out, lse, w
 
 
 def token_weights(q, k_cache, softmax_lse, cu_seqlens_q, max_seqlen_q, cache_seqlens, block_table, weights, softmax_scale,
                   is_causal=True, decay=1.0, weights_out=None):
     """fa_b200_token_weights: weight of every cached key under a prompt's queries, into ``weights_out`` (None: ``weights``)."""
+    if _grad():
+        _forward_only(q, k_cache)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
     ks, kst, index = _check_cache(k_cache, "token_weights")
     ts, t_stride = _check_tables(block_table, cache_seqlens, index, "token_weights")
     qs, qst = q.shape, q.stride()
@@ -1555,6 +1594,8 @@ def token_weights(q, k_cache, softmax_lse, cu_seqlens_q, max_seqlen_q, cache_seq
 def kv_evict(k_cache, v_cache, block_table, cache_seqlens, weights, budget, sink_tokens, recent_tokens,
              new_block_table=None, weights_out=None):
     """fa_b200_kv_evict: (kept_index (b, h_k, budget), new lengths (b))."""
+    if _grad():
+        _forward_only(k_cache, v_cache)
     ks, kst, index = _check_cache(k_cache, "kv_evict", v_cache)
     ts, t_stride = _check_tables(block_table, cache_seqlens, index, "kv_evict")
     nb, page, h_k, d = ks
