@@ -424,7 +424,8 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       float sum = 0.f, comp = 0.f;
       // what the sum is added to, on its way during the steps
       const bool adds = p.w_in && p.num_chunks == 1 && col0 == 0 && key < w.s.len && key < p.capacity;
-      const float before = adds ? p.w_in[w.b * p.win_b + w.hk * p.win_h + key] * p.decay : 0.f;
+      float before = 0.f;   // no use of it up here: a load that is on its way
+      if (adds) asm volatile("ld.global.f32 %0, [%1];" : "=f"(before) : "l"(p.w_in + w.b * p.win_b + w.hk * p.win_h + key));
       // the steps of this half: those whose last query sees its first key
       int j = 0;
       const int tile_step = p.num_chunks * p.tile_tokens;
@@ -482,7 +483,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (p.num_chunks > 1)
           p.partial[((static_cast<int64_t>(w.chunk) * p.b + w.b) * p.h_k + w.hk) * p.partial_stride + key] = sum;
         else if (key < p.capacity)
-          p.w_out[w.b * p.wout_b + w.hk * p.wout_h + key] = before + sum;
+          p.w_out[w.b * p.wout_b + w.hk * p.wout_h + key] = fmaf(before, p.decay, sum);
       }
     }
     __syncwarp();
