@@ -90,7 +90,13 @@ __global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const KvEvictP
   for (int i = kept + tid; i < p.budget; i += kPickThreads) out[i] = -1;
 }
 
-// A warp moves kMoveVectors * 32 / (16-byte vectors of a row) rows at a time: a lane looks up where one of them comes from
+// Rows that a warp moves at a time: what kMoveVectors vectors per lane hold, and no more than it has lanes to look them up.
+__host__ __device__ constexpr int move_rows(int row_bytes) {
+  const int rows = 32 / (row_bytes >> 4) * kMoveVectors;
+  return rows < 32 ? rows : 32;
+}
+
+// A warp moves move_rows rows at a time: a lane looks up where one of them comes from
 // and goes to, then all lanes load kMoveVectors vectors each, rows side by side, and store them.
 // blockIdx: x kv head and K / V (fastest: the heads of a token lie side by side, and their kept positions are near each
 // other), y piece of the kept rows (one CTA walks all pieces in place), z sequence.
@@ -110,9 +116,9 @@ __global__ void __launch_bounds__(kMoveMaxThreads) evict_move_kernel(const KvEvi
   const int dst_max = in_place ? p.max_blocks : p.new_max_blocks;
   uint8_t* pool = static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + hk * (is_v ? p.v_h : p.k_h);
   const int64_t blk = is_v ? p.v_blk : p.k_blk, row = is_v ? p.v_row : p.k_row;
-  const int nv = p.row_bytes >> 4;                                   // 16-byte vectors of a row: 8, 16, 24 or 32
+  const int nv = p.row_bytes >> 4;                                   // 16-byte vectors of a row: 4 to 32
   const int side = 32 / nv;                                          // rows side by side
-  const int rows = side * kMoveVectors;                              // of a warp at a time, at most 32
+  const int rows = move_rows(p.row_bytes);                           // of a warp at a time
   const int r_in = lane / nv, vec = lane - r_in * nv;
   const int piece = rows * (blockDim.x >> 5);
   for (int first = blockIdx.y * piece; first < kept; first += gridDim.y * piece) {
@@ -135,13 +141,13 @@ __global__ void __launch_bounds__(kMoveMaxThreads) evict_move_kernel(const KvEvi
 #pragma unroll
     for (int u = 0; u < kMoveVectors; ++u) {
       const int64_t s = __shfl_sync(0xffffffffu, from, (u * side + r_in) & 31);
-      if (s >= 0 && r_in < side) v[u] = *reinterpret_cast<const uint4*>(pool + s + vec * 16);
+      if (s >= 0 && r_in < side && u * side < rows) v[u] = *reinterpret_cast<const uint4*>(pool + s + vec * 16);
     }
     if (in_place) __syncthreads();
 #pragma unroll
     for (int u = 0; u < kMoveVectors; ++u) {
       const int64_t d = __shfl_sync(0xffffffffu, to, (u * side + r_in) & 31);
-      if (d >= 0 && r_in < side) *reinterpret_cast<uint4*>(pool + d + vec * 16) = v[u];
+      if (d >= 0 && r_in < side && u * side < rows) *reinterpret_cast<uint4*>(pool + d + vec * 16) = v[u];
     }
   }
 }
@@ -166,7 +172,7 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const bool in_place = p.new_block_table == nullptr;
   const int threads = in_place ? kMoveMaxThreads : kMoveThreads;
-  const int piece = 32 / (p.row_bytes >> 4) * kMoveVectors * (threads / 32);
+  const int piece = move_rows(p.row_bytes) * (threads / 32);
   cfg.gridDim = dim3(p.h_k * 2, in_place ? 1 : (p.budget + piece - 1) / piece, p.b);
   cfg.blockDim = dim3(threads);
   return cudaLaunchKernelEx(&cfg, evict_move_kernel, p);

@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t topk_border(int want, Each each, TopkShared&
     if (k == ~0u) ++sure;
     else if (k != 0u) { lo = min(lo, k); hi = max(hi, k); }
   });
-  if (tid == 0) { sh.lo = ~0u; sh.hi = 0u; sh.sure = 0; }
+  if (tid == 0) { sh.lo = ~0u; sh.hi = 0u; sh.sure = 0; sh.bin = 0; sh.above = 0; sh.in_bin = 0; }
   __syncthreads();
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t topk_border(int want, Each each, TopkShared&
     return ~0u;
   }
   want -= sh.sure;
-  while (true) {
+  for (int pass = 0; pass < 5; ++pass) {   // 32 bits, ten at a time: four at most (values that change meanwhile end it too)
     const uint32_t span = hi - lo;
     const int shift = max(0, 32 - __clz(span) - 10);   // span >> shift < kTopkBins
 #pragma unroll
@@ -121,11 +121,10 @@ __device__ __forceinline__ uint32_t topk_border(int want, Each each, TopkShared&
       take_equal = 0;
       return lo - 1u;
     }
-    if (shift == 0) {
-      take_equal = want;
-      return lo;
-    }
+    if (shift == 0) break;
   }
+  take_equal = want;
+  return lo;
 }
 
 // Running numbers of the chosen.

@@ -205,6 +205,9 @@ def kvcache_evict(
     ``token_weights_out`` of the same capacity) become zero from the new to the old length.  Page bounds of the pages written
     have to be made anew.
 
+    token_weights has to cover the lengths (capacity >= cache_seqlens; shorter ones cut the sequence, which device_status
+    reports).
+
     Returns (kept_index, new_seqlens): kept_index int32 (batch, nheads_k, budget) the kept positions, ascending, -1 behind
     them; new_seqlens int32 (batch,) = min(cache_seqlens, budget)."""
     if recent_tokens is None:

@@ -302,7 +302,9 @@ def test_decode_weights_from_nothing_and_short_capacity(fa):
     (HF, 128, 15, 3, 16, True, [257, 64, 200], [32, 7, 1], True),
     (BF, 64, 8, 8, 32, True, [700], None, False), (HF, 192, 8, 1, 128, True, [400, 130], [300, 0], False),
     (BF, 256, 4, 4, 64, False, [129, 260], [40, 260], True), (HF, 128, 16, 1, 64, False, [500], [33], False),
-    (BF, 128, 7, 7, 256, True, [1100], None, False), (BF, 128, 40, 1, 64, True, [333], [100], False)])
+    (BF, 128, 7, 7, 256, True, [1100], None, False), (BF, 128, 40, 1, 64, True, [333], [100], False),
+    (HF, 64, 128, 1, 64, True, [140, 70], [9, 70], False),                 # one token per query tile
+    (BF, 128, 4, 2, 16, True, [1, 130, 0, 257] * 40, [1, 5, 0, 8] * 40, True)])   # a batch of short windows
 def test_token_weights_of_a_prompt(fa, dtype, d, h, h_k, page, causal, lens, nq, bhsd):
     m, cuda = fa
     g = gen(9)
@@ -361,7 +363,8 @@ def test_token_weights_of_a_long_prompt(fa):
 @pytest.mark.parametrize("dtype,d,h_k,page,budget,sink,recent,in_place,bhsd", [
     (BF, 128, 4, 64, 200, 4, 50, False, False), (HF, 64, 2, 16, 333, 0, 0, True, False), (BF, 256, 1, 128, 1, 1, 0, False, True),
     (HF, 192, 3, 32, 64, 0, 64, True, True), (F8, 128, 2, 64, 500, 16, 100, True, False), (BF, 128, 8, 64, 1024, 4, 256, True, False),
-    (torch.float8_e5m2, 128, 2, 256, 257, 3, 7, False, False)])
+    (torch.float8_e5m2, 128, 2, 256, 257, 3, 7, False, False), (F8, 64, 2, 64, 300, 4, 40, False, False),
+    (torch.float8_e5m2, 192, 1, 16, 300, 4, 40, True, False)])
 def test_evict(fa, dtype, d, h_k, page, budget, sink, recent, in_place, bhsd):
     m, cuda = fa
     g = gen(11)
