@@ -12,6 +12,7 @@ namespace fa {
 namespace {
 
 constexpr int kPickThreads = 1024;
+constexpr int kPickSmemKeys = 48 * 1024;
 constexpr int kMoveThreads = 256, kMoveMaxThreads = 1024;   // into new pages; in place, where one CTA does all
 constexpr int kMoveVectors = 8;    // 16-byte vectors in flight per thread
 
@@ -25,11 +26,12 @@ __device__ __forceinline__ int evict_len(const KvEvictParams& p, int bi, bool re
   return len;
 }
 
-// V keys in a row per thread; IN_REGS: the row's keys stay in registers (up to V * kPickThreads tokens), else they are read
-// again for every pass.
-template <int V, bool IN_REGS>
-__global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const KvEvictParams p) {
+// IN_SMEM: the row's keys stay in shared memory (up to kPickSmemKeys tokens; two CTAs per SM up to 16384), else they are made
+// again from the weights for every pass.  Four keys in a row per thread at a time.
+template <bool IN_SMEM>
+__global__ void __launch_bounds__(kPickThreads, IN_SMEM ? 2 : 1) evict_pick_kernel(const KvEvictParams p) {
   __shared__ TopkShared sh;
+  extern __shared__ uint4 sm_keys[];
   const int hk = blockIdx.x, bi = blockIdx.y, tid = threadIdx.x;
   griddep_wait();
   griddep_launch_dependents();
@@ -45,42 +47,49 @@ __global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const KvEvictP
       if (wo != w) wo[i] = w[i];
     }
   } else {
-    auto load = [&](int i0, uint32_t (&k)[V], float (&x)[V]) {   // keys i0 .. i0 + V - 1; 0: past the end
-      if (i0 + V <= len && (reinterpret_cast<uintptr_t>(w + i0) & 15) == 0) {
-#pragma unroll
-        for (int j = 0; j < V; j += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(w + i0 + j);
-          x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
-        }
+    const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+    auto make = [&](int i0) -> uint4 {   // keys i0 .. i0 + 3; 0: past the end
+      float x[4];
+      if (i0 + 4 <= len && aligned) {
+        const float4 v = *reinterpret_cast<const float4*>(w + i0);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = i0 + j < len ? w[i0 + j] : 0.f;
+        for (int j = 0; j < 4; ++j) x[j] = i0 + j < len ? w[i0 + j] : 0.f;
       }
+      uint32_t k[4];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < 4; ++j) {
         const int i = i0 + j;
         k[j] = i >= len ? 0u : ((i < p.sink || i >= len - p.recent) ? ~0u : order_key(x[j]));
       }
+      return make_uint4(k[0], k[1], k[2], k[3]);
     };
-    constexpr int kTile = V * kPickThreads;
-    uint32_t k[V];
-    float x[V];
-    if (IN_REGS) load(tid * V, k, x);
+    const int quads = (len + 3) >> 2;
+    if (IN_SMEM) {   // a thread reads back what it wrote
+#pragma unroll 4
+      for (int q = tid; q < quads; q += kPickThreads) sm_keys[q] = make(4 * q);
+    }
+    auto quad = [&](int q) -> uint4 { return IN_SMEM ? sm_keys[q] : make(4 * q); };
     int take_equal;
-    const uint32_t border = topk_border<kPickThreads>(kept, [&](auto f) {
-      for (int i0 = 0; i0 < len; i0 += kTile) {
-        if (!IN_REGS) load(i0 + tid * V, k, x);
-#pragma unroll
-        for (int j = 0; j < V; ++j) f(k[j]);
+    const uint32_t border = topk_border<kPickThreads>(kept, p.sink + p.recent, [&](auto f) {
+      for (int q = tid; q < quads; q += kPickThreads) {
+        const uint4 k = quad(q);
+        f(k.x); f(k.y); f(k.z); f(k.w);
       }
     }, sh, take_equal);
     // the weights move with the keys, tile by tile: a tile's weights are read before topk_place's barriers, and the
     // positions written lie at or below the ones read
     TopkCount base;
-    for (int i0 = 0; i0 < len; i0 += kTile) {
-      if (!IN_REGS) load(i0 + tid * V, k, x);
-      topk_place<kPickThreads, V>(k, border, take_equal, base, sh, [&](int j, int at) {
-        out[at] = i0 + tid * V + j;
+    for (int q0 = 0; q0 < quads; q0 += kPickThreads) {
+      const int q = q0 + tid;
+      const uint4 v = q < quads ? quad(q) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t k[4] = {v.x, v.y, v.z, v.w};
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = k[j] >= border && k[j] != 0u ? w[4 * q + j] : 0.f;
+      topk_place<kPickThreads, 4>(k, border, take_equal, base, sh, [&](int j, int at) {
+        out[at] = 4 * q + j;
         wo[at] = x[j];
       });
     }
@@ -165,10 +174,22 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = p.dependent_launch ? 1 : 0;
   const int64_t most = min(static_cast<int64_t>(p.max_blocks) * p.page_size, static_cast<int64_t>(p.capacity));
-  cudaError_t e = most <= 4 * kPickThreads    ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<4, true>, p)
-                  : most <= 8 * kPickThreads  ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<8, true>, p)
-                  : most <= 16 * kPickThreads ? cudaLaunchKernelEx(&cfg, evict_pick_kernel<16, true>, p)
-                                              : cudaLaunchKernelEx(&cfg, evict_pick_kernel<8, false>, p);
+  cudaError_t e;
+  if (most <= kPickSmemKeys) {
+    static bool attr_done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !attr_done[dev]) {
+      e = cudaFuncSetAttribute(evict_pick_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickSmemKeys * 4);
+      if (e != cudaSuccess) return e;
+      if (dev < 64) attr_done[dev] = true;
+    }
+    cfg.dynamicSmemBytes = static_cast<size_t>(most + 3) / 4 * 16;
+    e = cudaLaunchKernelEx(&cfg, evict_pick_kernel<true>, p);
+    cfg.dynamicSmemBytes = 0;
+  } else {
+    e = cudaLaunchKernelEx(&cfg, evict_pick_kernel<false>, p);
+  }
   if (e != cudaSuccess) return e;
   const bool in_place = p.new_block_table == nullptr;
   const int threads = in_place ? kMoveMaxThreads : kMoveThreads;

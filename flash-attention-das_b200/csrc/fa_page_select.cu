@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const PageS
       }
     };
     int take_equal;
-    uint32_t border = topk_border<kSelectThreads>(chosen, [&](auto f) { each([&](uint32_t x, int) { f(x); }); }, sh, take_equal);
+    uint32_t border = topk_border<kSelectThreads>(chosen, -1, [&](auto f) { each([&](uint32_t x, int) { f(x); }); }, sh, take_equal);
     // The lowest score taken and the highest one left: the 32-bit choice stands if they differ by more than both errors.
     uint32_t lowest = ~0u, highest = 0u;
     each([&](uint32_t x, int) {

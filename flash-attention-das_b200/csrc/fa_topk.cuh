@@ -24,12 +24,13 @@ __device__ __forceinline__ uint64_t order_key(double x) {
 // The value of a key (of ~0: a NaN).
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
-constexpr int kTopkBins = 1024;
+constexpr int kTopkBins = 1024, kTopkList = 2048;
 struct TopkShared {
   int hist[kTopkBins];
+  uint32_t list[kTopkList];
   int warp_total[32];
   uint32_t lo, hi;
-  int sure, bin, above, in_bin;
+  int sure, bin, above, in_bin, listed;
 };
 
 // Sum of x over the threads before this one; `total`: over all.
@@ -61,46 +62,57 @@ __device__ __forceinline__ int block_exclusive(int x, TopkShared& sh, int& total
 // keys (0: no key; ~0: always taken).
 //
 // Every pass counts the keys between two bounds in kTopkBins equal steps and goes on in the step that holds the border, or
-// ends when that step's keys are all wanted.  The first bounds are the smallest and largest key, so a row whose values
-// share their leading bits costs no pass for them: keys that differ need two passes, whatever their distribution is like
-// three or four.
+// ends when that step's keys are all wanted; once a step's keys fit a short list, the passes that follow read that.
+// sure < 0: the first bounds are the smallest and largest key, so a row whose values share their leading bits costs no pass
+// for them (but a look at every key first).  sure >= 0: the number of keys that are always taken; the first steps are half a
+// power of two of a 32-bit value wide.
 template <int THREADS, class Each>
-__device__ __forceinline__ uint32_t topk_border(int want, Each each, TopkShared& sh, int& take_equal) {
+__device__ __forceinline__ uint32_t topk_border(int want, int sure, Each each, TopkShared& sh, int& take_equal) {
   constexpr int kPer = kTopkBins / THREADS;
   static_assert(kPer * THREADS == kTopkBins, "whole bins per thread");
   const int tid = threadIdx.x, lane = tid & 31;
-  uint32_t lo = ~0u, hi = 0u;
-  int sure = 0;
-  each([&](uint32_t k) {
-    if (k == ~0u) ++sure;
-    else if (k != 0u) { lo = min(lo, k); hi = max(hi, k); }
-  });
-  if (tid == 0) { sh.lo = ~0u; sh.hi = 0u; sh.sure = 0; sh.bin = 0; sh.above = 0; sh.in_bin = 0; }
-  __syncthreads();
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  sure = __reduce_add_sync(0xffffffffu, sure);
-  if (lane == 0) {
-    atomicMin(&sh.lo, lo);
-    atomicMax(&sh.hi, hi);
-    atomicAdd(&sh.sure, sure);
+  uint32_t lo = 1u, hi = ~0u - 1u;
+  if (tid == 0) { sh.lo = ~0u; sh.hi = 0u; sh.sure = 0; sh.bin = 0; sh.above = 0; sh.in_bin = 0; sh.listed = 0; }
+  if (sure < 0) {
+    lo = ~0u; hi = 0u;
+    int count = 0;
+    each([&](uint32_t k) {
+      if (k == ~0u) ++count;
+      else if (k != 0u) { lo = min(lo, k); hi = max(hi, k); }
+    });
+    __syncthreads();
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0) {
+      atomicMin(&sh.lo, lo);
+      atomicMax(&sh.hi, hi);
+      atomicAdd(&sh.sure, count);
+    }
+    __syncthreads();
+    lo = sh.lo; hi = sh.hi;
+    sure = sh.sure;
   }
-  __syncthreads();
-  lo = sh.lo; hi = sh.hi;
-  if (want <= sh.sure) {
+  if (want <= sure) {
     take_equal = want;
     return ~0u;
   }
-  want -= sh.sure;
+  want -= sure;
+  bool listed = false;
   for (int pass = 0; pass < 5; ++pass) {   // 32 bits, ten at a time: four at most (values that change meanwhile end it too)
     const uint32_t span = hi - lo;
     const int shift = max(0, 32 - __clz(span) - 10);   // span >> shift < kTopkBins
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sh.hist[tid + j * THREADS] = 0;
     __syncthreads();
-    each([&](uint32_t k) {
-      if (k >= lo && k <= hi && k != ~0u) atomicAdd(&sh.hist[(k - lo) >> shift], 1);
-    });
+    auto count = [&](uint32_t k) {
+      if (k - lo <= span && k != ~0u) atomicAdd(&sh.hist[(k - lo) >> shift], 1);
+    };
+    if (listed) {
+      for (int i = tid; i < sh.listed; i += THREADS) count(sh.list[i]);
+    } else {
+      each(count);
+    }
     __syncthreads();
     int own[kPer], sum = 0, total;
 #pragma unroll
@@ -122,6 +134,17 @@ __device__ __forceinline__ uint32_t topk_border(int want, Each each, TopkShared&
       return lo - 1u;
     }
     if (shift == 0) break;
+    if (!listed && sh.in_bin <= kTopkList) {
+      const uint32_t range = hi - lo;
+      each([&](uint32_t k) {
+        if (k - lo <= range && k != ~0u) {
+          const int at = atomicAdd(&sh.listed, 1);
+          if (at < kTopkList) sh.list[at] = k;
+        }
+      });
+      listed = true;
+      __syncthreads();
+    }
   }
   take_equal = want;
   return lo;
