@@ -43,61 +43,25 @@ __host__ __device__ constexpr TwLayout tw_layout() {
   return s;
 }
 
-// Groups of four columns, of the eight in 32, whose exponentials go to the FMA pipe instead of the MUFU unit.  Measured on one
-// prompt of 8192 tokens (32 heads, 8 kv heads, bf16): none 408 us, one group 397, two 416, three 444: the kernel is bound by
-// the instructions it issues nearly as much as by the MUFU unit.
-constexpr int kPolyGroups = 0x10;
-// 2^x of two values on the FMA pipe: round-to-nearest range reduction by the magic-number add, a degree-5 polynomial of 2^f
-// on [-0.5, 0.5] (weighted least squares towards the minimax, constant term 1; relative error 9.2e-8, 1.7e-7 with its 32-bit
-// rounding), the integer part added to the exponent field.  x is clamped to [-127, 128], where that gives exactly 0 and
-// infinity: with the constant term 1 no mantissa falls below 1 at the lower end.
-__device__ __forceinline__ void exp2_poly2(uint64_t x, float& p0, float& p1) {
-  float x0, x1;
-  unpack_f32x2(x, x0, x1);
-  x0 = fminf(fmaxf(x0, -127.f), 128.f);
-  x1 = fminf(fmaxf(x1, -127.f), 128.f);
-  const uint64_t x2 = pack_f32x2(x0, x1);
-  const uint64_t t2 = add_f32x2(x2, pack_f32x2(12582912.f, 12582912.f));   // 1.5 * 2^23: the low mantissa bits hold round(x)
-  const uint64_t r2 = add_f32x2(t2, pack_f32x2(-12582912.f, -12582912.f));
-  const uint64_t f2 = fma_f32x2(r2, pack_f32x2(-1.f, -1.f), x2);
-  uint64_t q2 = fma_f32x2(f2, pack_f32x2(0.001326472731307149f, 0.001326472731307149f), pack_f32x2(0.009671512991189957f, 0.009671512991189957f));
-  q2 = fma_f32x2(q2, f2, pack_f32x2(0.05550733581185341f, 0.05550733581185341f));
-  q2 = fma_f32x2(q2, f2, pack_f32x2(0.24022242426872253f, 0.24022242426872253f));
-  q2 = fma_f32x2(q2, f2, pack_f32x2(0.6931470036506653f, 0.6931470036506653f));
-  q2 = fma_f32x2(q2, f2, pack_f32x2(1.f, 1.f));
-  float q0, q1, t0, t1;
-  unpack_f32x2(q2, q0, q1);
-  unpack_f32x2(t2, t0, t1);
-  p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
-  p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
-}
-
-// Sum of 2^(scale s + neg_lse) over the columns [c_first, c_end) of COLS columns of an S^T row; MASK false: all of them.
-// `release` runs once the row has been read from TMEM.
-template <bool MASK, int COLS, class Release>
+// Sum of 2^(scale s + neg_lse) over the columns [c_first, c_end) of an S^T row; MASK false: all 128 columns.  `release` runs
+// once the row has been read from TMEM.
+template <bool MASK, class Release>
 __device__ __forceinline__ float tile_sum(uint32_t t_s, const float* neg_lse, float scale, int c_first, int c_end, Release release) {
   const uint64_t sc2 = pack_f32x2(scale, scale);
   uint64_t acc0 = 0ull, acc1 = 0ull;
 #pragma unroll 1
-  for (int ch = 0; ch < COLS / 32; ++ch) {   // a loop, for the instruction cache
+  for (int ch = 0; ch < 4; ++ch) {   // a loop, for the instruction cache
     uint32_t v[32];
     tmem_ld_32x32(t_s + ch * 32, v);
     tmem_wait_ld();
-    if (ch == COLS / 32 - 1) release();
+    if (ch == 3) release();
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       const float4 l = *reinterpret_cast<const float4*>(neg_lse + ch * 32 + i);
-      const uint64_t xa = fma_f32x2(pack_f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, pack_f32x2(l.x, l.y));
-      const uint64_t xb = fma_f32x2(pack_f32x2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2, pack_f32x2(l.z, l.w));
       float x0, x1, x2, x3;
-      if (!MASK && ((kPolyGroups >> (i / 4)) & 1)) {
-        exp2_poly2(xa, x0, x1);
-        exp2_poly2(xb, x2, x3);
-      } else {
-        unpack_f32x2(xa, x0, x1);
-        unpack_f32x2(xb, x2, x3);
-        x0 = fast_exp2(x0); x1 = fast_exp2(x1); x2 = fast_exp2(x2); x3 = fast_exp2(x3);
-      }
+      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, pack_f32x2(l.x, l.y)), x0, x1);
+      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2, pack_f32x2(l.z, l.w)), x2, x3);
+      x0 = fast_exp2(x0); x1 = fast_exp2(x1); x2 = fast_exp2(x2); x3 = fast_exp2(x3);
       if (MASK) {   // a column that holds no visible query may hold anything
         const int c = ch * 32 + i;
         x0 = (c >= c_first && c < c_end) ? x0 : 0.f;
@@ -136,7 +100,7 @@ __device__ __forceinline__ TwSeq tw_seq(const TokenWeightsParams& p, int b) {
 // One CTA's walk over its items and their query tiles.  KEYS: keys of an item.
 template <int KEYS>
 struct TwWalk {
-  int item, end, stride;         // items left
+  int item, end, round;          // this item, the share's end (resident) or the batch's, rounds of the grid
   int b, base, here;             // sequence, its first item, its number of items
   int key_tiles;
   TwSeq s;
@@ -150,7 +114,13 @@ struct TwWalk {
   // Moves to the next query tile, or the next item (steps may be 0: no query sees its keys).  false: done.
   __device__ __forceinline__ bool next(const TokenWeightsParams& p) { return ++j < steps || next_item(p); }
   __device__ __forceinline__ bool next_item(const TokenWeightsParams& p) {
-    item += stride;
+    if (p.resident) {
+      ++item;
+    } else {                       // back and forth, so that no CTA has the heavier item of every round
+      const int g = gridDim.x;
+      item = round * g + ((round & 1) ? g - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+      ++round;
+    }
     if (item >= end) return false;
     while (item >= base + here) {
       base += here;
@@ -182,11 +152,9 @@ struct TwWalk {
       const int64_t g = gridDim.x;
       item = static_cast<int>(total * static_cast<int64_t>(blockIdx.x) / g) - 1;
       end = static_cast<int>(total * static_cast<int64_t>(blockIdx.x + 1) / g);
-      stride = 1;
     } else {
-      item = static_cast<int>(blockIdx.x) - static_cast<int>(gridDim.x);
+      round = 0;
       end = total;
-      stride = gridDim.x;
     }
     base = 0; steps = 0; j = 0;
     enter(p, 0);
@@ -240,7 +208,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   using T = TileTraits<DT, HD>;
   constexpr TwLayout L = tw_layout<DT, HD>();
   constexpr int kTiles = tw_tiles(HD), kHalvesOfKeys = tw_halves(HD), kProducer = 8, kMma = 9;
-  constexpr int kSplit = 2 / kHalvesOfKeys, kColsOfWarp = 128 / kSplit, kLaneCols = kColsOfWarp / 32;
+  constexpr bool kTurns = kHalvesOfKeys == 1;     // two sets of four warps take turns at the tiles of one set of keys
   constexpr int kCols = 256 * kHalvesOfKeys;   // TMEM
   constexpr int kForever = 0x7fffffff;
   extern __shared__ uint8_t smem_raw[];
@@ -265,7 +233,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&s_full[i]), 1);
-      mbar_init(smem_u32(&s_empty[i]), 128 * kSplit);
+      mbar_init(smem_u32(&s_empty[i]), 128);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmap_q);
@@ -395,89 +363,95 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
     __syncwarp();
   } else {
-    // key half * 128 + row of the item's, columns col0 .. of every tile
-    const int half = kSplit == 1 ? warp >> 2 : 0, row = threadIdx.x & 127, col0 = kSplit == 1 ? 0 : (warp >> 2) * kColsOfWarp;
-    // this lane's columns, whose log-sum-exp it fetches for the warp: token and head
-    int t_in[kLaneCols];
-    int64_t h_off[kLaneCols];
+    // Key half * 128 + row of the item's.  kTurns: set 0 takes the even steps of the CTA's walk and set 1 the odd ones (each
+    // has one S^T buffer), so that one set's exponentials fill the other's waits; the sums meet at the item's end.  Items of
+    // one step (resident) belong to one set.
+    const int set = warp >> 2, half = kTurns ? 0 : set, row = threadIdx.x & 127;
+    // this lane's four columns, whose log-sum-exp it fetches for the warp: token and head
+    int t_in[4];
+    int64_t h_off[4];
 #pragma unroll
-    for (int e = 0; e < kLaneCols; ++e) {
-      const int c = col0 + lane * kLaneCols + e;
+    for (int e = 0; e < 4; ++e) {
+      const int c = lane * 4 + e;
       t_in[e] = c / p.group;
       h_off[e] = static_cast<int64_t>(c - t_in[e] * p.group) * p.lse_h + t_in[e];
     }
     float* sm_lse = reinterpret_cast<float*>(smem + L.lse_off) + warp * 256;   // this warp's own: [2][128]
-    float* sm_sum = reinterpret_cast<float*>(smem + L.lse_off) + 8 * 256;      // [2][128]: sums of the second warp of a pair
-    const uint32_t t_s = tmem_base + half * 256 + col0 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    float* sm_sum = reinterpret_cast<float*>(smem + L.lse_off) + 8 * 256;      // [2][128]: sums of set 1
+    const uint32_t t_s = tmem_base + half * 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     TwWalk<128 * kHalvesOfKeys> w{};
-    int t = 0, q_key = -1, items = 0;
+    int t = 0, q_key = -1, items = 0, stage = 0;   // t: the CTA's steps before this item (kTurns), or this half's
     bool ok = true;
-    float next[kLaneCols];       // log-sum-exp of the lane's columns in the tile to come; +inf: no query
+    float next[4];       // log-sum-exp of the lane's columns in the tile to come; +inf: no query
     const float* lse = nullptr;
     auto fetch = [&](int tok0) {
 #pragma unroll
-      for (int e = 0; e < kLaneCols; ++e)
+      for (int e = 0; e < 4; ++e)
         next[e] = (t_in[e] < p.tile_tokens && tok0 + t_in[e] < w.s.n) ? __ldg(lse + h_off[e] + tok0) : INFINITY;
     };
-    for (bool more = w.begin(p, total); more; more = w.next_item(p)) {   // after an abort the pairs still meet, item by item
+    const int tile_step = p.num_chunks * p.tile_tokens * (kTurns ? 2 : 1);
+    for (bool more = w.begin(p, total); more; more = w.next_item(p)) {   // after an abort the sets still meet, item by item
       const int key = w.k0 + half * 128 + row;
       float sum = 0.f, comp = 0.f;
-      // what the sum is added to, on its way during the steps
-      const bool adds = p.w_in && p.num_chunks == 1 && col0 == 0 && key < w.s.len && key < p.capacity;
-      float before = 0.f;   // no use of it up here: a load that is on its way
-      if (adds) asm volatile("ld.global.f32 %0, [%1];" : "=f"(before) : "l"(p.w_in + w.b * p.win_b + w.hk * p.win_h + key));
-      // the steps of this half: those whose last query sees its first key
-      int j = 0;
-      const int tile_step = p.num_chunks * p.tile_tokens;
-      if (half > 0) {
+      int j = 0;   // first step of this set or half
+      if (kTurns) {
+        j = (set ^ t) & 1;
+        if (p.resident && (w.steps > 0 ? j : set) != 0) {   // the other set's item
+          t += w.steps;
+          continue;
+        }
+      } else if (half > 0) {   // steps whose last query sees the half's first key
         if (!w.second()) continue;
         if (p.causal)
           while (j < w.steps && w.first * p.tile_tokens + j * tile_step + p.tile_tokens <= w.k0 + 128 - (w.s.len - w.s.n)) ++j;
       }
-      int tile0 = w.first * p.tile_tokens + j * tile_step;
+      // what the sum is added to, on its way during the steps
+      const bool writes = !kTurns || p.resident || set == 0;
+      const bool adds = p.w_in && p.num_chunks == 1 && writes && key < w.s.len && key < p.capacity;
+      float before = 0.f;   // no use of it up here: a load that is on its way
+      if (adds) asm volatile("ld.global.f32 %0, [%1];" : "=f"(before) : "l"(p.w_in + w.b * p.win_b + w.hk * p.win_h + key));
+      int tile0 = (w.first + j * p.num_chunks) * p.tile_tokens;
       if (j < w.steps && (!p.resident || w.b * p.h_k + w.hk != q_key)) {
         q_key = w.b * p.h_k + w.hk;
         lse = p.lse + static_cast<int64_t>(w.hk) * p.group * p.lse_h + w.s.q0;
         fetch(tile0);
       }
       int ahead = key - (w.s.len - w.s.n) - tile0;   // this key's position relative to the tile's first query
-      for (; j < w.steps && ok; ++j, tile0 += tile_step, ahead -= tile_step) {
-        const int buf = t & 1;
-        // a log-sum-exp that is not finite goes with scores that may not be: the exponentials that keep infinities and NaN
-        bool plain = true;
-#pragma unroll
-        for (int e = 0; e < kLaneCols; ++e) {
-          plain = plain && fabsf(next[e]) < INFINITY;
-          sm_lse[buf * 128 + lane * kLaneCols + e] = -next[e] * kLog2e;
-        }
-        if (j + 1 < w.steps) fetch(tile0 + tile_step);
-        const int c_first = (p.causal ? max(0, min(ahead, p.tile_tokens)) * p.group : 0) - col0;
-        const int c_end = min(p.tile_tokens, w.s.n - tile0) * p.group - col0;
-        const bool mask = c_end < kColsOfWarp || __any_sync(0xffffffffu, c_first > 0 || !plain);
+      for (; j < w.steps && ok; j += kTurns ? 2 : 1, tile0 += tile_step, ahead -= tile_step) {
+        const int step = kTurns ? t + j : t, buf = step & 1;
+        stage ^= 128;
+        float4 neg;
+        neg.x = -next[0] * kLog2e; neg.y = -next[1] * kLog2e; neg.z = -next[2] * kLog2e; neg.w = -next[3] * kLog2e;
+        *reinterpret_cast<float4*>(sm_lse + stage + lane * 4) = neg;
+        if (j + (kTurns ? 2 : 1) < w.steps) fetch(tile0 + tile_step);
+        const int c_end = min(p.tile_tokens, w.s.n - tile0) * p.group;
+        const int c_first = p.causal ? max(0, min(ahead, p.tile_tokens)) * p.group : 0;
+        const bool mask = c_end < 128 || __any_sync(0xffffffffu, c_first > 0);
         __syncwarp();
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[2 * half + buf]), (t >> 1) & 1, wctx));
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[2 * half + buf]), (step >> 1) & 1, wctx));
         if (!ok) break;
         tc_fence_after();
         auto release = [&] {
           tc_fence_before();
           mbar_arrive(smem_u32(&s_empty[2 * half + buf]));
         };
-        const float part = mask ? tile_sum<true, kColsOfWarp>(t_s + buf * 128, sm_lse + buf * 128, p.scale_log2, c_first, c_end, release)
-                                : tile_sum<false, kColsOfWarp>(t_s + buf * 128, sm_lse + buf * 128, p.scale_log2, 0, kColsOfWarp, release);
+        const float part = mask ? tile_sum<true>(t_s + buf * 128, sm_lse + stage, p.scale_log2, c_first, c_end, release)
+                                : tile_sum<false>(t_s + buf * 128, sm_lse + stage, p.scale_log2, 0, 128, release);
         // up to tens of thousands of queries: the total carries its rounding errors along
         const float now = __fadd_rn(sum, part);
         const float big = fmaxf(sum, part), small = fminf(sum, part);
         comp = __fadd_rn(comp, __fsub_rn(small, __fsub_rn(now, big)));
         sum = now;
-        ++t;
+        if (!kTurns) ++t;
       }
+      if (kTurns) t += w.steps;
       sum += comp;
-      if constexpr (kSplit == 2) {   // the pair's second warp hands its sums over; two buffers, so one meeting per item
-        sm_sum += items++ & 1 ? -128 : 128;
-        if (col0 > 0) sm_sum[row] = sum;
+      if (kTurns && !p.resident) {   // two buffers, so one meeting per item
+        float* s = sm_sum + (items++ & 1) * 128;
+        if (set == 1) s[row] = sum;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
-        if (col0 > 0) continue;
-        sum += sm_sum[row];
+        if (set == 1) continue;
+        sum += s[row];
       }
       if (ok && key < w.s.len) {
         if (p.num_chunks > 1)
