@@ -6,19 +6,24 @@
 // S^T = K Q^T in TMEM.  A TMEM lane is then a key, so a key's sum stays in a thread's registers: no atomics, no second pass.
 // A query tile holds 128 / group tokens of all heads of the group (rows token-major), which fills it for short windows too
 // and makes the causal mask a column bound per key.
-//   warps 0-7  one thread per key and half of a tile's columns (above d = 128: per key of 256): 2^(s - lse) and its sum
+//   warps 0-7  2^(s - lse) and its sum, one thread per key: two sets of four warps that take turns at the tiles (above
+//              d = 128: one set for each 128 keys)
 //   warp 8     TMA producer: key tiles (through the block table) and query tiles into a pool of tile buffers
-//   warp 9     MMA issuer, two S^T buffers per 128 keys
+//   warp 9     MMA issuer, an S^T buffer per set (two above d = 128)
 // Two persistent CTAs per SM (one above d = 128) walk the items (key tiles, kv head, share of the query tiles) of the batch,
-// so that the loads and the first product of an item run during the sums of the one before.  Long prompts: items go round
-// robin, heaviest first under a causal mask, and a key tile's query tiles are cut into shares (every num_chunks-th tile),
-// whose sums a small kernel adds in order.  Short windows (one query tile per sequence): a CTA takes consecutive key tiles
-// and keeps the query tile, which leaves the keys as the only traffic.
+// so that the loads and the first product of an item run during the sums of the one before.  Long prompts: items go back and
+// forth over the CTAs, heaviest first under a causal mask, and a key tile's query tiles are cut into shares (every
+// num_chunks-th tile), whose sums a small kernel adds in order.  Short windows (one query tile per sequence): a CTA takes
+// consecutive key tiles and keeps the query tile, which leaves the keys as the only traffic.
 //
-// Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit, its tcgen05 product 256.
-// One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128, causal): 397 us, 69 % of what the MUFU units could do at the
-// 1.7 GHz that the GPU ran at.  One CTA per SM with 256 keys, which halves the query traffic, measured 536 us, eight warps per SM
-// instead of sixteen 436 us, a CTA per key tile 424 us.  32 queries against 4 x 16384 keys: a CTA per key tile 78 us.
+// Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit; the tcgen05 product takes 512,
+// as long as its two operands take out of shared memory.  One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128, causal):
+// 391 us, 70 % of what the MUFU units could do at the 1.7 GHz that the GPU ran at; a CTA per key tile 424 us, one CTA per SM with
+// 256 keys 536, eight warps per SM 436, two warps per row with half of the columns each 408, the issuing threads walking
+// through a general plan of the buffers 404.  Exponentials on the FMA pipe (a degree-5 polynomial) cost more issue slots than
+// the MUFU time they save: one group of columns in eight 416 us against 404.  A quarter of the columns for four rows per thread
+// (16x256b loads) halves the shared-memory reads of the log-sum-exps and measured 399 against 404, but the registers that it
+// takes cost short windows 50 us against 43.  32 queries against 4 x 16384 keys (134 MB of keys): 38 us; a CTA per key tile 78.
 #include "fa_prefill_common.cuh"
 
 namespace fa {
@@ -29,9 +34,9 @@ namespace {
 // MUFU unit busier than 8 do).
 __host__ __device__ constexpr int tw_halves(int hd) { return hd > 128 ? 2 : 1; }
 constexpr int kTwThreads = 320;
-constexpr int kTwMaxTiles = 6;
+constexpr int kTwMaxTiles = 4;
 // Tile buffers for keys and queries.
-__host__ __device__ constexpr int tw_tiles(int hd) { return hd == 64 ? 6 : (hd == 192 ? 4 : 3); }
+__host__ __device__ constexpr int tw_tiles(int hd) { return hd == 192 ? 4 : 3; }
 struct TwLayout { int lse_off, bar_off, misc_off, total; };
 template <int DT, int HD>
 __host__ __device__ constexpr TwLayout tw_layout() {
@@ -261,7 +266,109 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const int total = *sm_total;
   const uint32_t tiles_smem = smem_u32(smem);
 
-  if (warp == kProducer) {
+  // Up to d = 128 (kTurns) the three tile buffers go round by rule: an item's keys take the buffer that has been out of use
+  // longest, its query tiles alternate between the other two; resident: the keys alternate between 0 and 1, the query tile
+  // stays in 2.  `loaded` has the parity of every buffer's number of loads.
+  if (kTurns && warp == kProducer) {
+    if (lane == 0) {
+      TwWalk<128> w{};
+      int t = 0, q_key = -1, k = 0, q0 = 1, q1 = 2;
+      uint32_t loaded = 0, used = 0;
+      const uint32_t q_bytes = static_cast<uint32_t>(p.tile_tokens) * p.group * 128u * T::kHalves;
+      bool ok = true;
+      auto reserve = [&](int slot) {
+        if ((used >> slot) & 1u) ok = ok && mbar_wait(smem_u32(&empty[slot]), ((loaded >> slot) & 1u) ^ 1u, wctx);
+        if (!ok) return;
+        loaded ^= 1u << slot;
+        used |= 1u << slot;
+      };
+      for (bool more = w.begin(p, total); more && ok; more = w.next_item(p)) {
+        if (w.steps == 0) continue;
+        if (p.resident) k = t & 1;
+        {
+          // the page ids are looked up before the wait for a buffer
+          const int nbox = min(128 / p.box_rows, (w.s.len - w.k0 + p.box_rows - 1) / p.box_rows);
+          const int32_t* bt = p.block_table + w.b * p.bt_stride;
+          int page[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) page[i] = i < nbox ? __ldg(bt + (w.k0 + i * p.box_rows) / p.page_size) : 0;
+          reserve(k);
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&full[k]);
+          mbar_expect_tx(bar, static_cast<uint32_t>(nbox) * p.box_rows * 128u * T::kHalves);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i >= nbox) break;
+            const int row = (w.k0 + i * p.box_rows) % p.page_size;
+#pragma unroll
+            for (int hf = 0; hf < T::kHalves; ++hf)
+              tma_load_4d(tiles_smem + k * T::kTileBytes + hf * T::kHalfBytes + i * p.box_rows * 128, &tmap_k, bar, hf * 64, w.hk, row, page[i]);
+          }
+        }
+        const int key = w.b * p.h_k + w.hk;
+        int tok = w.s.q0 + w.first * p.tile_tokens;
+        for (int j = 0; j < w.steps && ok; ++j, tok += p.num_chunks * p.tile_tokens) {
+          if (p.resident && key == q_key) continue;
+          const int slot = p.resident ? 2 : ((j & 1) ? q1 : q0);
+          reserve(slot);
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&full[slot]);
+          mbar_expect_tx(bar, q_bytes);
+#pragma unroll
+          for (int hf = 0; hf < T::kHalves; ++hf)
+            tma_load_4d(tiles_smem + slot * T::kTileBytes + hf * T::kHalfBytes, &tmap_q, bar, hf * 64, w.hk * p.group, tok, 0);
+        }
+        q_key = key;
+        t += w.steps;
+        const int last = (w.steps & 1) ? q0 : q1, other = (w.steps & 1) ? q1 : q0, old_k = k;
+        k = other; q0 = old_k; q1 = last;
+      }
+      if (!ok)   // gave up: the loads issued last may still be on their way
+        for (int i = 0; i < 3; ++i)
+          if ((used >> i) & 1u) drain(smem_u32(&full[i]), ((loaded >> i) & 1u) ^ 1u);
+    }
+  } else if (kTurns && warp == kMma) {
+    if (lane == 0) {
+      TwWalk<128> w{};
+      int t = 0, q_key = -1, k = 0, q0 = 1, q1 = 2;
+      uint32_t loaded = 0;
+      bool ok = true;
+      auto landed = [&](int slot) {   // the next load of a buffer
+        loaded ^= 1u << slot;
+        ok = ok && mbar_wait(smem_u32(&full[slot]), ((loaded >> slot) & 1u) ^ 1u, wctx);
+      };
+      for (bool more = w.begin(p, total); more && ok; more = w.next_item(p)) {
+        if (w.steps == 0) continue;
+        const int key = w.b * p.h_k + w.hk;
+        if (p.resident) {
+          k = t & 1;
+          if (key != q_key) {
+            if (q_key >= 0) tc_commit(smem_u32(&empty[2]));   // the products that read the old query tile have been issued
+            landed(2);
+          }
+        }
+        q_key = key;
+        landed(k);
+        for (int j = 0; j < w.steps && ok; ++j, ++t) {
+          const int slot = p.resident ? 2 : ((j & 1) ? q1 : q0), buf = t & 1;
+          if (!p.resident) landed(slot);
+          ok = ok && mbar_wait(smem_u32(&s_empty[buf]), ((t >> 1) & 1) ^ 1u, wctx);
+          if (!ok) break;
+          tc_fence_after();
+          issue_qk<DT, HD>(tiles_smem + k * T::kTileBytes, tiles_smem + slot * T::kTileBytes, tmem_base + buf * 128);
+          tc_commit(smem_u32(&s_full[buf]));
+          if (!p.resident) tc_commit(smem_u32(&empty[slot]));
+        }
+        if (!ok) break;
+        tc_commit(smem_u32(&empty[k]));
+        const int last = (w.steps & 1) ? q0 : q1, other = (w.steps & 1) ? q1 : q0, old_k = k;
+        k = other; q0 = old_k; q1 = last;
+      }
+      if (!ok)     // gave up: products in flight end before TMEM is freed
+        for (int i = max(0, t - 2); i < t; ++i) drain(smem_u32(&s_full[i & 1]), (i >> 1) & 1);
+    }
+    __syncwarp();
+  } else if (warp == kProducer) {
     if (lane == 0) {
       TwWalk<128 * kHalvesOfKeys> w{};
       TwBuffers<kTiles> buf;
