@@ -147,7 +147,7 @@ def flash_attn_with_kvcache_weights(
         raise RuntimeError("token_weights or token_weights_out is required")
     out, lse, w = flash_attn_cuda.decode_budget(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, causal,
                                                 out, s_aux, window_size[0], token_weights, token_weights_out,
-                                                decay, q_descale, k_descale, v_descale)
+                                                decay, q_descale, k_descale, v_descale, True)
     return (out, lse, w) if return_softmax_lse else (out, w)
 
 

@@ -11,12 +11,12 @@ It keeps the reference binding's function names, positional argument order and r
     fwd_sparse   -> [out, softmax_lse]  (flash_api_sparse.cpp:170-338)
 
 PyTorch is used for what the reference binding used ATen for: output / scratch allocation on the input's
-device and the current stream.  All compute happens in the library's sm_100a kernels; there is no CPU or
+device and the current stream (the bounded-cache calls do that part in C++, csrc/fa_host.cpp).  All compute happens in the library's sm_100a kernels; there is no CPU or
 eager fallback — if the shared library is missing the import fails.
 """
 import ctypes
+import importlib.util
 import os
-import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -317,6 +317,7 @@ def set_profile_events(start: Optional["torch.cuda.Event"], stop: Optional["torc
     right before and right after its main kernel, so the dominant kernel can be timed alone."""
     global _profile_events
     _profile_events = None if start is None else (start, stop)
+    _host.set_profile_events(*((0, 0) if start is None else (start.cuda_event, stop.cuda_event)))
 
 
 def _own_work_counter(p, device):
@@ -375,12 +376,8 @@ def last_launch_info() -> str:
 _KERNEL_CHOICE = {"single": 1, "pair": 2, "dense": 3}
 
 
-_environ = getattr(os.environ, "_data", None)      # the mapping behind os.environ: no encoding of the name per look
-_PARTITION = os.environ.encodekey("FA_B200_DECODE_PARTITION") if _environ is not None else None
-
-
 def _env_partition() -> int:
-    v = os.environ.get("FA_B200_DECODE_PARTITION") if _environ is None else _environ.get(_PARTITION)
+    v = os.environ.get("FA_B200_DECODE_PARTITION")
     return int(v) if v else 0
 
 
@@ -1292,331 +1289,29 @@ def block_select(pooled_q, pooled_k, sim_q, sim_k, block_q, block_k, scale, cdf_
 # ------------------------------------------------------------------------------------------------
 # decode with a bounded KV cache
 # ------------------------------------------------------------------------------------------------
-# A decode step makes several of these calls with a few microseconds of GPU work each, so what the host spends per call
-# counts: every tensor is asked for its shape, strides and device once, and a parameter struct is packed in one go.
-_DT_CACHE = {**_DT, torch.float8_e5m2: 4}
-_HALF = (torch.float16, torch.bfloat16)
-_FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
-
-
-def _packer(cls, fmt):
-    """struct.Struct of a parameter struct, native alignment (P: pointer, q: int64, i / I: int32, f: float, N: size_t)."""
-    s = struct.Struct("@" + fmt + "0q")
-    assert s.size == ctypes.sizeof(cls), cls.__name__
-    return s
-
-
-_PACK_BOUNDS = _packer(PageBoundsParams, "IPqqqPPqPiiiiiiiii")
-_PACK_SELECT = _packer(PageSelectParams, "IPqqqPPqPPPPiiiiiiiiiiiiPN")
-_PACK_DECODE = _packer(DecodeParams, "IPPPPPqqqqqqqqqqPqPiiiiiiifiiPPPqqqqqqiiPNPPPPPiiiiiiqqiiP")
-_PACK_BUDGET = _packer(DecodeBudgetParams, "IiqPPqqqqif")
-_PACK_WEIGHTS = _packer(TokenWeightsParams, "IPqqPqPPqqqPqPPPqqqqifqiiiiiiiifiiPN")
-_PACK_EVICT = _packer(KvEvictParams, "IPPqqqqqqPqPqPPPqqqqiPPiiiiiiiiiii")
-
-
-def _raw(name, *argtypes, restype=ctypes.c_int):
-    """The library's function as one that takes packed structs (bytes)."""
-    f = _lib[name]
-    f.argtypes, f.restype = argtypes, restype
-    return f
-
-
-_cc = ctypes.c_char_p
-_page_bounds_raw = _raw("fa_b200_page_bounds", _cc, _c_vp)
-_page_select_raw = _raw("fa_b200_page_select", _cc, _c_vp)
-_page_select_bytes = _raw("fa_b200_page_select_workspace_bytes", _cc, restype=ctypes.c_size_t)
-_decode_budget_raw = _raw("fa_b200_decode_budget", _cc, _cc, _c_vp)
-_decode_budget_bytes = _raw("fa_b200_decode_budget_workspace_bytes", _cc, _cc, restype=ctypes.c_size_t)
-_token_weights_raw = _raw("fa_b200_token_weights", _cc, _c_vp)
-_token_weights_bytes = _raw("fa_b200_token_weights_workspace_bytes", _cc, restype=ctypes.c_size_t)
-_kv_evict_raw = _raw("fa_b200_kv_evict", _cc, _c_vp)
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
-_grad = torch.is_grad_enabled
-_ERR_WORKSPACE = 8
-
-
-def _run_on(index, what, call, size):
-    """``call(workspace pointer, workspace bytes, stream)`` with device ``index`` current.  Outside stream capture the
-    (device, stream)'s cached scratch is offered and grown if the library refuses it as too small (before any launch);
-    ``size(pointer, bytes)`` asks how much there has to be.  size None: a call without scratch."""
-    before = _current_device()
-    if before != index:
-        torch.cuda.set_device(index)
+# page_bounds, page_select, decode_budget, token_weights and kv_evict over the C ABI's functions of those names.  A decode step
+# makes several of these calls with a few microseconds of GPU work each, so their host part (checks, outputs, scratch, the
+# parameter struct) is compiled: csrc/fa_host.cpp, which lists the arguments, all positional.
+def _load_host():
+    path = os.path.join(_HERE, "_fa_b200_host.so")
+    rebuild = f"build it with `python {os.path.join(_HERE, 'build.py')} --force`"
+    if not os.path.exists(path):
+        raise ImportError(f"{path} not found: {rebuild} (there is no fallback implementation)")
+    spec = importlib.util.spec_from_file_location("_fa_b200_host", path)
     try:
-        stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
-        if size is None:
-            status = call(0, 0, stream)
-        elif _capturing():
-            need = size(0, 0)
-            ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index)) if need else None
-            status = call(0 if ws is None else ws.data_ptr(), need, stream)
-        else:
-            ws = _workspaces.get((index, stream))
-            status = call(0, 0, stream) if ws is None else call(ws.data_ptr(), ws.numel(), stream)
-            if status == _ERR_WORKSPACE:
-                ws = _workspace(torch.device("cuda", index), size(0, 0))
-                status = call(ws.data_ptr(), ws.numel(), stream)
-        if status != 0:
-            _check(status, what)
-    finally:
-        if before != index:
-            torch.cuda.set_device(before)
+        host = importlib.util.module_from_spec(spec)
+    except ImportError as e:
+        raise ImportError(f"{path} does not load with torch {torch.__version__}: {rebuild}") from e
+    spec.loader.exec_module(host)
+    if torch.__version__.split("+")[0] != host.TORCH_VERSION:
+        raise ImportError(f"{path} was built for torch {host.TORCH_VERSION}, this is {torch.__version__}: {rebuild}")
+    host.bind(tuple(ctypes.cast(_lib[name], _c_vp).value for name in host.FUNCTIONS))
+    return host
 
 
-def _forward_only(*tensors):
-    if any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError("the B200 hot path is forward only: call under torch.no_grad() or detach inputs")
-
-
-def _check_tables(block_table, cache_seqlens, index, what):
-    """Shape and strides of an int32 block table (b, n) with the lengths (b) beside it, on device ``index``."""
-    s, st = block_table.shape, block_table.stride()
-    if not (len(s) == 2 and block_table.dtype is torch.int32 and block_table.get_device() == index and (st[1] == 1 or s[1] <= 1)):
-        _require(False, f"{what}: block_table must be an int32 tensor (batch, max_num_blocks_per_seq) on the cache's device with "
-                 "contiguous last dimension")
-    if not (cache_seqlens.dtype is torch.int32 and cache_seqlens.get_device() == index and cache_seqlens.shape == s[:1] and
-            cache_seqlens.is_contiguous()):
-        _require(False, f"{what}: cache_seqlens must be a contiguous int32 tensor (batch,) on the cache's device")
-    return s, st[0]
-
-
-def _check_cache(k_cache, what, v_cache=None):
-    """Shape, strides and device index of a paged pool (num_blocks, page, h_k, d) with d contiguous."""
-    s, st, index = k_cache.shape, k_cache.stride(), k_cache.get_device()
-    if not (index >= 0 and len(s) == 4 and st[3] == 1):
-        _require(False, f"{what}: k_cache must be a CUDA tensor (num_blocks, page_size, nheads_k, d) with contiguous last dimension")
-    if k_cache.dtype not in _DT_CACHE:
-        _require(False, f"{what}: the cache must be fp16, bf16, fp8 e4m3 or fp8 e5m2")
-    if v_cache is not None and not (v_cache.shape == s and v_cache.dtype == k_cache.dtype and v_cache.get_device() == index and
-                                    v_cache.stride(3) == 1):
-        _require(False, f"{what}: v_cache must be like k_cache, with contiguous last dimension")
-    return s, st, index
-
-
-def _weights_args(w_in, w_out, b, h_k, index, what):
-    """fp32 token weights (b, h_k, capacity), capacity contiguous; w_out None: in place.  (w_out, the struct's fields)."""
-    if w_out is None:
-        _require(w_in is not None, f"{what}: token_weights is required")
-        w_out = w_in
-    s, st = w_out.shape, w_out.stride()
-    same = w_in is None or w_in is w_out
-    ok = w_out.dtype is torch.float32 and w_out.get_device() == index and len(s) == 3 and s[0] == b and s[1] == h_k and \
-        (st[2] == 1 or s[2] <= 1)
-    if ok and not same:
-        st_in = w_in.stride()
-        ok = w_in.dtype is torch.float32 and w_in.get_device() == index and w_in.dim() == 3 and (st_in[2] == 1 or s[2] <= 1)
-    if not ok:
-        _require(False, f"{what}: token weights must be a float32 tensor (batch, nheads_k, capacity) on the cache's device with "
-                 "contiguous last dimension")
-    if same:
-        st_in = st
-    elif w_in.shape != s:
-        _require(False, f"{what}: token_weights_out must have the shape of token_weights")
-    return w_out, (0 if w_in is None else w_in.data_ptr(), w_out.data_ptr(), st_in[0], st_in[1], st[0], st[1], s[2])
-
-
-def page_bounds(k_cache, block_table, cache_seqlens, bounds, new_tokens=0):
-    """fa_b200_page_bounds: writes ``bounds`` (num_blocks, h_k, 2, d), fp16 / bf16."""
-    if _grad():
-        _forward_only(k_cache)
-    s, st, index = _check_cache(k_cache, "page_bounds")
-    ts, t_stride = _check_tables(block_table, cache_seqlens, index, "page_bounds")
-    nb, page, h_k, d = s
-    if not (bounds.shape == (nb, h_k, 2, d) and bounds.is_contiguous() and bounds.get_device() == index and bounds.dtype in _HALF and
-            (k_cache.dtype in _FP8 or bounds.dtype == k_cache.dtype)):
-        _require(False, "page_bounds: bounds must be a contiguous tensor (num_blocks, nheads_k, 2, d) of the cache's type (fp16 or bf16 "
-                 "for an fp8 cache) on the cache's device")
-    p = _PACK_BOUNDS.pack(_PACK_BOUNDS.size, k_cache.data_ptr(), st[0], st[1], st[2], bounds.data_ptr(), block_table.data_ptr(), t_stride,
-                          cache_seqlens.data_ptr(), ts[0], h_k, d, page, nb, ts[1], new_tokens, _DT_CACHE[k_cache.dtype], _DT[bounds.dtype])
-    _run_on(index, "page_bounds", lambda ws, n, stream: _page_bounds_raw(p, stream), None)
-    return bounds
-
-
-def page_select(q, bounds, block_table, cache_seqlens, page_size, num_pages, sink_pages=1, recent_pages=1):
-    """fa_b200_page_select: (page_table, seqlens, page_index)."""
-    if _grad():
-        _forward_only(q, bounds)
-    qs, qst, index = q.shape, q.stride(), q.get_device()
-    if qst[-1] != 1:
-        q = q.contiguous()
-        qst = q.stride()
-    if not (index >= 0 and len(qs) == 4 and qst[3] == 1 and q.dtype in _HALF):
-        _require(False, "page_select: q must be an fp16 / bf16 CUDA tensor (batch, seqlen_q, nheads, d) with contiguous last dimension")
-    b, sq, h, d = qs
-    bs = bounds.shape
-    if not (len(bs) == 4 and bs[2] == 2 and bs[3] == d and bounds.is_contiguous() and bounds.dtype == q.dtype and bounds.get_device() == index):
-        _require(False, "page_select: page_bounds must be a contiguous tensor (num_blocks, nheads_k, 2, d) of q's type on q's device")
-    ts, t_stride = _check_tables(block_table, cache_seqlens, index, "page_select")
-    _require(ts[0] == b, "page_select: block_table batch mismatch")
-    _require(num_pages > 0, "page_select: num_pages must be positive")
-    h_k = bs[1]
-    table, pages = q.new_empty((2, b, h_k, num_pages), dtype=torch.int32).unbind(0)
-    lens = q.new_empty((b, h_k), dtype=torch.int32)
-    head = (_PACK_SELECT.size, q.data_ptr(), qst[0], qst[1], qst[2], bounds.data_ptr(), block_table.data_ptr(), t_stride,
-            cache_seqlens.data_ptr(), table.data_ptr(), pages.data_ptr(), lens.data_ptr(), b, sq, h, h_k, d, page_size, bs[0], ts[1], num_pages,
-            sink_pages, recent_pages, _DT[q.dtype])
-    pack = _PACK_SELECT.pack
-    _run_on(index, "page_select", lambda ws, n, stream: _page_select_raw(pack(*head, ws, n), stream),
-            lambda ws, n: _page_select_bytes(pack(*head, ws, n)))
-    return table, lens, pages
-
-
-def _descale_args(name, t, b, h_k):
-    """Pointer and strides of an fp32 descale of one element or shape (batch, h_k)."""
-    if t is None:
-        return 0, 0, 0
-    _require(t.dtype is torch.float32 and t.is_cuda, f"{name} must be a float32 CUDA tensor")
-    if t.numel() == 1:
-        return t.data_ptr(), 0, 0
-    _require(t.dim() == 2 and t.shape[0] == b and t.shape[1] == h_k, f"{name} must have one element or shape (batch, nheads_k)")
-    return t.data_ptr(), t.stride(0), t.stride(1)
-
-
-def decode_budget(q, kcache, vcache, block_table, seqlens, softmax_scale, is_causal=False, out=None, s_aux=None,
-                  window_left=-1, token_weights=None, token_weights_out=None, decay=1.0, q_descale=None, k_descale=None,
-                  v_descale=None, need_lse=True):
-    """fa_b200_decode_budget: decode over the pages of ``block_table`` (b, n), or (b, h_k, n) with ``seqlens`` (b, h_k), and,
-    when token weights are given, the weight of every key.  Returns (out, softmax_lse, token weights or None)."""
-    if _grad():
-        _forward_only(q, kcache, vcache)
-    vst = vcache.stride()
-    if len(vst) == 4 and vst[3] != 1 and vst[1] == 1:
-        _unsupported(True, "a transposed V pool (layout 0)")
-    ks, kst, index = _check_cache(kcache, "decode_budget", vcache)
-    qs, qst, qt, kt = q.shape, q.stride(), q.dtype, kcache.dtype
-    if qst[-1] != 1:
-        q = q.contiguous()
-        qst = q.stride()
-    fp8_kv = qt in _HALF and kt in _FP8
-    if not (len(qs) == 4 and qst[3] == 1 and q.get_device() == index):
-        _require(False, "q must be a CUDA tensor (batch, seqlen_q, nheads, d) on the caches' device with contiguous last dimension")
-    if not (qt in _DT and (fp8_kv or kt == qt)):
-        _require(qt in _DT, "FlashAttention only support fp16, bf16 and fp8 e4m3 data type")
-        _require(False, "query and key must have the same dtype")
-    b, sq, h, d = qs
-    nb, page, h_k, dk = ks
-    _require(dk == d, "query and key must have the same head dimension")
-    _require(h % h_k == 0, "Number of heads in key/value must divide number of heads in query")
-    _require(sq >= 1, "q must hold at least one token per sequence")
-    if fp8_kv and q_descale is not None:
-        _unsupported(True, "an fp8 KV cache under 16-bit queries with q_descale")
-    ts, tst, ls = block_table.shape, block_table.stride(), seqlens.shape
-    if tst[-1] != 1 and ts[-1] > 1:
-        block_table = block_table.contiguous()
-        tst = block_table.stride()
-    per_head = len(ts) == 3
-    if not (block_table.dtype is torch.int32 and block_table.get_device() == index and (tst[-1] == 1 or ts[-1] <= 1) and
-            ts[:-1] == ((b, h_k) if per_head else (b,))):
-        _require(False, "the block table must be int32, (batch, n) or (batch, nheads_k, n), on q's device with contiguous last dimension")
-    if not (seqlens.dtype is torch.int32 and seqlens.get_device() == index and ls == ts[:-1] and seqlens.is_contiguous()):
-        _require(False, "the lengths must be a contiguous int32 tensor, (batch,) or with a table for each kv head (batch, nheads_k)")
-    if out is not None:
-        odt = _out_dtype(q, out)
-        _require(out.shape == qs and out.stride(-1) == 1 and out.get_device() == index,
-                 "out must have the shape of q and a contiguous last dimension")
-    elif qt in _HALF and q.is_contiguous():
-        out, odt = torch.empty_like(q), qt
-    else:
-        odt = _out_dtype(q, None)
-        out = q.new_empty(qs, dtype=odt)
-    lse = q.new_empty((b, h, sq), dtype=torch.float32) if need_lse else None
-    w = None
-    if token_weights is not None or token_weights_out is not None:
-        w, (wi, wo, wi_b, wi_h, wo_b, wo_h, capacity) = _weights_args(token_weights, token_weights_out, b, h_k, index, "token weights")
-        e = _PACK_BUDGET.pack(_PACK_BUDGET.size, per_head, tst[1] if per_head else 0, wi, wo, wi_b, wi_h, wo_b, wo_h, capacity, decay)
-    else:
-        e = _PACK_BUDGET.pack(_PACK_BUDGET.size, per_head, tst[1] if per_head else 0, 0, 0, 0, 0, 0, 0, 0, 1.0)
-    qd = kd = vd = (0, 0, 0)
-    if q_descale is not None:
-        qd = _descale_args("q_descale", q_descale, b, h_k)
-    if k_descale is not None:
-        kd = _descale_args("k_descale", k_descale, b, h_k)
-    if v_descale is not None:
-        vd = _descale_args("v_descale", v_descale, b, h_k)
-    sink, sink_dt = 0, 0
-    if s_aux is not None:
-        s_aux = s_aux.contiguous()
-        holder = DecodeParams()
-        _set_sinks(holder, s_aux, h)
-        sink, sink_dt = holder.s_aux, holder.s_aux_dtype
-    ev0, ev1 = (0, 0) if _profile_events is None else (_profile_events[0].cuda_event, _profile_events[1].cuda_event)
-    ost = out.stride()
-
-    def params(ws, n):
-        return _PACK_DECODE.pack(
-            _PACK_DECODE.size, q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), qst[0],
-            qst[2], ost[0], ost[2], kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], block_table.data_ptr(), tst[0], seqlens.data_ptr(), b, h, h_k,
-            d, nb, page, ts[-1], softmax_scale, _DT[qt], _DT[odt], qd[0], kd[0], vd[0], qd[1], qd[2], kd[1], kd[2], vd[1], vd[2],
-            _env_partition(), 0, ws, n, 0, 0, ev0, ev1, sink, sink_dt, window_left >= 0, window_left, 0, sq, bool(is_causal), qst[1], ost[1],
-            fp8_kv, fp8_kv and kt is torch.float8_e5m2, 0)
-
-    _run_on(index, "decode_budget", lambda ws, n, stream: _decode_budget_raw(params(ws, n), e, stream),
-            lambda ws, n: _decode_budget_bytes(params(ws, n), e))
-    return out, lse, w
-
-
-def token_weights(q, k_cache, softmax_lse, cu_seqlens_q, max_seqlen_q, cache_seqlens, block_table, weights, softmax_scale,
-                  is_causal=True, decay=1.0, weights_out=None):
-    """fa_b200_token_weights: weight of every cached key under a prompt's queries, into ``weights_out`` (None: ``weights``)."""
-    if _grad():
-        _forward_only(q, k_cache)
-    if q.stride(-1) != 1:
-        q = q.contiguous()
-    ks, kst, index = _check_cache(k_cache, "token_weights")
-    ts, t_stride = _check_tables(block_table, cache_seqlens, index, "token_weights")
-    qs, qst = q.shape, q.stride()
-    if not (len(qs) == 3 and q.get_device() == index and qst[2] == 1):
-        _require(False, "token_weights: q must be (total_q, nheads, d) on the cache's device with contiguous last dimension")
-    if q.dtype not in _HALF or k_cache.dtype != q.dtype:
-        _unsupported(True, "token_weights with other than fp16 or bf16 queries and a cache of their type")
-    total_q, h, d = qs
-    nb, page, h_k, dk = ks
-    b = ts[0]
-    _require(dk == d and h % h_k == 0, "token_weights: q and k_cache must have the same d, and nheads_k must divide nheads")
-    lst = softmax_lse.stride()
-    if not (softmax_lse.dtype is torch.float32 and softmax_lse.get_device() == index and softmax_lse.shape == (h, total_q) and
-            (lst[1] == 1 or total_q <= 1)):
-        _require(False, "token_weights: softmax_lse must be a float32 tensor (nheads, total_q) with contiguous last dimension")
-    if not (cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.get_device() == index and cu_seqlens_q.is_contiguous() and
-            cu_seqlens_q.shape == (b + 1,)):
-        _require(False, "token_weights: cu_seqlens_q must be a contiguous int32 tensor (batch + 1,)")
-    w, weight_args = _weights_args(weights, weights_out, b, h_k, index, "token_weights")
-    head = (_PACK_WEIGHTS.size, q.data_ptr(), qst[0], qst[1], softmax_lse.data_ptr(), lst[0], cu_seqlens_q.data_ptr(), k_cache.data_ptr(), kst[0],
-            kst[1], kst[2], block_table.data_ptr(), t_stride, cache_seqlens.data_ptr(), *weight_args, decay, total_q, b, max_seqlen_q, h, h_k, d,
-            page, nb, ts[1], softmax_scale, bool(is_causal), _DT[q.dtype])
-    pack = _PACK_WEIGHTS.pack
-    _run_on(index, "token_weights", lambda ws, n, stream: _token_weights_raw(pack(*head, ws, n), stream),
-            lambda ws, n: _token_weights_bytes(pack(*head, ws, n)))
-    return w
-
-
-def kv_evict(k_cache, v_cache, block_table, cache_seqlens, weights, budget, sink_tokens, recent_tokens,
-             new_block_table=None, weights_out=None):
-    """fa_b200_kv_evict: (kept_index (b, h_k, budget), new lengths (b))."""
-    if _grad():
-        _forward_only(k_cache, v_cache)
-    ks, kst, index = _check_cache(k_cache, "kv_evict", v_cache)
-    ts, t_stride = _check_tables(block_table, cache_seqlens, index, "kv_evict")
-    nb, page, h_k, d = ks
-    b = ts[0]
-    _require(budget > 0, "kv_evict: budget must be positive")
-    _require(weights is not None, "kv_evict: token_weights is required")
-    _, weight_args = _weights_args(weights, weights_out, b, h_k, index, "kv_evict")
-    new_ptr = new_stride = new_n = 0
-    if new_block_table is not None:
-        ns, nst = new_block_table.shape, new_block_table.stride()
-        _require(new_block_table.dtype is torch.int32 and len(ns) == 2 and new_block_table.get_device() == index and ns[0] == b and
-                 (nst[1] == 1 or ns[1] <= 1), "kv_evict: new_block_table must be like block_table")
-        new_ptr, new_stride, new_n = new_block_table.data_ptr(), nst[0], ns[1]
-    kept = k_cache.new_empty((b, h_k, budget), dtype=torch.int32)
-    lens = k_cache.new_empty((b,), dtype=torch.int32)
-    vst = v_cache.stride()
-    p = _PACK_EVICT.pack(_PACK_EVICT.size, k_cache.data_ptr(), v_cache.data_ptr(), kst[0], kst[1], kst[2], vst[0], vst[1], vst[2],
-                         block_table.data_ptr(), t_stride, new_ptr, new_stride, cache_seqlens.data_ptr(), *weight_args, kept.data_ptr(),
-                         lens.data_ptr(), b, h_k, d, page, nb, ts[1], new_n, budget, sink_tokens, recent_tokens, _DT_CACHE[k_cache.dtype])
-    _run_on(index, "kv_evict", lambda ws, n, stream: _kv_evict_raw(p, stream), None)
-    return kept, lens
+_host = _load_host()
+page_bounds, page_select, decode_budget = _host.page_bounds, _host.page_select, _host.decode_budget
+token_weights, kv_evict = _host.token_weights, _host.kv_evict
 
 
 # ------------------------------------------------------------------------------------------------

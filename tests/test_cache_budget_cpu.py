@@ -142,3 +142,20 @@ def test_python_refusals(binding):
     grad = z(2, 1, 8, 128).requires_grad_()
     with pytest.raises(NotImplementedError, match="forward only"):
         fa.sparse_attn_with_kvcache(grad, k, k, z(2, 2, 2, t=torch.int32), z(2, 2, t=torch.int32))
+
+
+def test_binding_argument_errors(binding):
+    """The compiled host part: wrong counts and kinds of arguments are Python errors, before anything else."""
+    k, i = torch.zeros(4, 64, 2, 128, dtype=torch.bfloat16), torch.zeros(2, 2, dtype=torch.int32)
+    with pytest.raises(TypeError, match="expected 5"):
+        binding.page_bounds(k, i)
+    with pytest.raises(TypeError, match="k_cache must be a tensor"):
+        binding.page_bounds(None, i, i, k, 0)
+    with pytest.raises(TypeError, match="new_block_table must be a tensor"):
+        binding.kv_evict(k, k, i, i[0], k.float(), 10, 0, 0, 3, None)
+    with pytest.raises(RuntimeError, match="token_weights is required"):
+        binding.kv_evict(k, k, i, i[0], None, 10, 0, 0, None, None)
+    with pytest.raises(RuntimeError, match="addresses"):
+        binding._host.bind((1, 2))
+    with pytest.raises(NotImplementedError, match="forward only"):
+        binding.page_bounds(k.clone().requires_grad_(), i, i[0], k, 0)
