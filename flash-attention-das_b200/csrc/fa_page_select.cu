@@ -198,8 +198,10 @@ __device__ __forceinline__ double row_score(const PageSelectParams& p, int bi, i
 // 2d 2^-23, per warp (with what may be flushed to zero, and infinity where it nears the end of the 32-bit range or is
 // no number); the choice below looks again in 64 bits at pages that are closer to the border.
 //
-// 32 sequences x 131072 tokens in pages of 64, 8 kv heads, 256 MB of bounds, bf16: 64-bit sums throughout took 148 us, 32-bit
-// multiply-adds on the FMA pipe 84 us (both bound by the instructions they issue).
+// 32 sequences x 131072 tokens in pages of 64, 8 kv heads, 256 MB of bounds, bf16: 51 us (5.2 TB/s; a CTA's start, which is a
+// chain of trips to memory, is what it is away from the copy rate), then 14 for the choice.  64-bit sums throughout took 148 us,
+// 32-bit multiply-adds on the FMA pipe 84 (both bound by the instructions they issue); four heads side by side in a CTA, one
+// warp each, or more stages with fewer CTAs per SM measured the same or slower.
 constexpr int kScoreWarps = 4;
 constexpr int kBatch = 8;          // pages of a warp at a time: the columns of one MMA tile
 constexpr int kScoreStages = 3;    // two batches in flight per warp while one is scored
@@ -208,9 +210,19 @@ constexpr int kMaxBatches = 32;
 __host__ __device__ constexpr bool a_in_regs(int hd) { return hd <= 128; }
 __host__ __device__ constexpr int score_smem(int hd) { return (a_in_regs(hd) ? 0 : hd / 8 * 512) + kScoreWarps * kScoreStages * kBatch * 4 * hd; }
 
-template <int DT> __device__ __forceinline__ uint32_t signed_part(uint32_t v, bool negative) {   // q- or q+ of two channels
-  const uint32_t neg = ((v & 0x8000u) ? 0xffffu : 0u) | ((v & 0x80000000u) ? 0xffff0000u : 0u);  // by the sign bit
-  return v & (negative ? neg : ~neg);
+// All ones in each half whose sign bit is set.
+__device__ __forceinline__ uint32_t sign_halves(uint32_t v) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// The larger magnitude of each half, with some sign; a NaN stays.  One instruction.
+template <int DT> __device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (DT == FA_B200_BF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // blockIdx: x kv head, y share of the pages, z sequence: the heads of a page, whose bounds lie side by side, are read at about
@@ -264,22 +276,30 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Page
   auto q_row = [&](int r) {
     return static_cast<const uint16_t*>(p.q) + bi * p.q_b + (r / p.group) * p.q_r + (static_cast<int64_t>(hk) * p.group + r % p.group) * p.q_h;
   };
-  auto fragments = [&](int c, uint4& a0, uint4& a1) {
-    const bool negative = c < kPieces / 2;
-    const int ch = (c % (kPieces / 2)) * 32 + qd * 8;
+  // Both the q- of piece c and the q+ of piece c + kPieces / 2.
+  const uint16_t* const q_g = q_row(g < rows ? g : 0) + qd * 8;
+  const uint16_t* const q_g8 = q_row(g + 8 < rows ? g + 8 : 0) + qd * 8;
+  auto fragments = [&](int c, uint4& n0, uint4& n1, uint4& p0, uint4& p1) {
     const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-    const uint4 r0 = g < rows ? *reinterpret_cast<const uint4*>(q_row(g) + ch) : z;
-    const uint4 r1 = g + 8 < rows ? *reinterpret_cast<const uint4*>(q_row(g + 8) + ch) : z;
-    auto f = [&](uint32_t v) { return signed_part<DT>(v, negative); };
-    a0 = make_uint4(f(r0.x), f(r1.x), f(r0.y), f(r1.y));
-    a1 = make_uint4(f(r0.z), f(r1.z), f(r0.w), f(r1.w));
+    const uint4 r0 = g < rows ? *reinterpret_cast<const uint4*>(q_g + c * 32) : z;
+    const uint4 r1 = g + 8 < rows ? *reinterpret_cast<const uint4*>(q_g8 + c * 32) : z;
+    const uint32_t v[8] = {r0.x, r1.x, r0.y, r1.y, r0.z, r1.z, r0.w, r1.w};
+    uint32_t n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n[i] = v[i] & sign_halves(v[i]);
+    n0 = make_uint4(n[0], n[1], n[2], n[3]);
+    n1 = make_uint4(n[4], n[5], n[6], n[7]);
+    p0 = make_uint4(v[0] ^ n[0], v[1] ^ n[1], v[2] ^ n[2], v[3] ^ n[3]);
+    p1 = make_uint4(v[4] ^ n[4], v[5] ^ n[5], v[6] ^ n[6], v[7] ^ n[7]);
   };
+  constexpr int kHalf = kPieces / 2;
   uint4 a[a_in_regs(HD) ? 2 * kPieces : 1];
   if constexpr (a_in_regs(HD)) {
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c) fragments(c, a[2 * c], a[2 * c + 1]);
+    for (int c = 0; c < kHalf; ++c) fragments(c, a[2 * c], a[2 * c + 1], a[2 * (c + kHalf)], a[2 * (c + kHalf) + 1]);
   } else {
-    for (int c = warp; c < kPieces; c += kScoreWarps) fragments(c, sm_a[(2 * c) * 32 + lane], sm_a[(2 * c + 1) * 32 + lane]);
+    for (int c = warp; c < kHalf; c += kScoreWarps)
+      fragments(c, sm_a[(2 * c) * 32 + lane], sm_a[(2 * c + 1) * 32 + lane], sm_a[(2 * (c + kHalf)) * 32 + lane], sm_a[(2 * (c + kHalf) + 1) * 32 + lane]);
   }
   for (int r = warp; r < rows; r += kScoreWarps) {   // sum |q_c| of every row
     float sum = 0.f;
@@ -296,7 +316,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Page
   for (int r = 0; r < rows; ++r) q1 = sm_q1[r] > q1 || isnan(sm_q1[r]) ? sm_q1[r] : q1;   // a NaN stays
   const int64_t pair = static_cast<int64_t>(bi) * p.h_k + hk;
   float* out = p.scores + pair * p.max_blocks;
-  uint32_t top = 0;   // largest magnitude: the bits of a 16-bit value without its sign order as the values do
+  uint32_t top = 0, top2 = 0;   // largest magnitudes, of either sign
   for (int n = 0; n < p.batches; ++n) {
     const int first = (first_batch + n * kScoreWarps) * kBatch;
     if (first >= s.pages) break;
@@ -318,10 +338,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Page
         mma_f16_16816(acc, f0, v.x, v.y);
         mma_f16_16816(acc2, f1, v.z, v.w);
       }
-      top = __vmaxu2(top, v.x & 0x7fff7fffu);
-      top = __vmaxu2(top, v.y & 0x7fff7fffu);
-      top = __vmaxu2(top, v.z & 0x7fff7fffu);
-      top = __vmaxu2(top, v.w & 0x7fff7fffu);
+      top = abs_max2<DT>(abs_max2<DT>(top, v.x), v.y);
+      top2 = abs_max2<DT>(abs_max2<DT>(top2, v.z), v.w);
     }
     // the largest of the rows g and g + 8 over g; columns 2 qd and 2 qd + 1
 #pragma unroll
@@ -334,9 +352,10 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Page
       if (g == 0 && first + slot < s.pages) out[first + slot] = ids[n * kScoreWarps * kBatch + slot] >= 0 ? v : -INFINITY;
     }
   }
+  top = abs_max2<DT>(top, top2);
 #pragma unroll
-  for (int st = 16; st > 0; st >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, st));
-  const float reach = q1 * Pair16<DT>::to_float(max(top & 0xffffu, top >> 16)).x;
+  for (int st = 16; st > 0; st >>= 1) top = abs_max2<DT>(top, __shfl_xor_sync(0xffffffffu, top, st));
+  const float reach = q1 * Pair16<DT>::to_float(max(top & 0x7fffu, (top >> 16) & 0x7fffu)).x;   // ordered by their bits; NaN on top
   if (lane == 0)   // not below 1e37: too large, or no number
     p.errors[pair * p.err_stride + chunk * kScoreWarps + warp] = reach < 1e37f ? reach * (1.1f * 2 * HD * 0x1p-23f) + 1e-35f : INFINITY;
   cp_async_wait<0>();
