@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(kPickThreads, IN_SMEM ? 2 : 1) evict_pick_kern
     }
   } else {
     const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+    const int inner_end = len - p.recent;
     auto make = [&](int i0) -> uint4 {   // keys i0 .. i0 + 3; 0: past the end
       float x[4];
       if (i0 + 4 <= len && aligned) {
@@ -59,9 +60,17 @@ __global__ void __launch_bounds__(kPickThreads, IN_SMEM ? 2 : 1) evict_pick_kern
       }
       uint32_t k[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j;
-        k[j] = i >= len ? 0u : ((i < p.sink || i >= len - p.recent) ? ~0u : order_key(x[j]));
+      for (int j = 0; j < 4; ++j) k[j] = __float_as_uint(x[j]);
+      // weights as they should be (0 to infinity, no -0) between the sinks and the recent tokens: a key is its bits, sign set
+      if (i0 >= p.sink && i0 + 4 <= inner_end && max(max(k[0], k[1]), max(k[2], k[3])) <= 0x7f800000u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] |= 0x80000000u;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = i0 + j;
+          k[j] = i >= len ? 0u : ((i < p.sink || i >= inner_end) ? ~0u : order_key(x[j]));
+        }
       }
       return make_uint4(k[0], k[1], k[2], k[3]);
     };
@@ -85,9 +94,12 @@ __global__ void __launch_bounds__(kPickThreads, IN_SMEM ? 2 : 1) evict_pick_kern
       const int q = q0 + tid;
       const uint4 v = q < quads ? quad(q) : make_uint4(0u, 0u, 0u, 0u);
       const uint32_t k[4] = {v.x, v.y, v.z, v.w};
-      float x[4];
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (max(max(k[0], k[1]), max(k[2], k[3])) >= border) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = k[j] >= border && k[j] != 0u ? w[4 * q + j] : 0.f;
+        for (int j = 0; j < 4; ++j)
+          if (k[j] >= border && k[j] != 0u) x[j] = w[4 * q + j];
+      }
       topk_place<kPickThreads, 4>(k, border, take_equal, base, sh, [&](int j, int at) {
         out[at] = 4 * q + j;
         wo[at] = x[j];

@@ -105,8 +105,8 @@ __device__ __forceinline__ uint32_t topk_border(int want, int sure, Each each, T
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sh.hist[tid + j * THREADS] = 0;
     __syncthreads();
-    auto count = [&](uint32_t k) {
-      if (k - lo <= span && k != ~0u) atomicAdd(&sh.hist[(k - lo) >> shift], 1);
+    auto count = [&](uint32_t k) {   // 0 and ~0 lie outside: 0 < lo, hi < ~0
+      if (k - lo <= span) atomicAdd(&sh.hist[(k - lo) >> shift], 1);
     };
     if (listed) {
       for (int i = tid; i < sh.listed; i += THREADS) count(sh.list[i]);
@@ -137,7 +137,7 @@ __device__ __forceinline__ uint32_t topk_border(int want, int sure, Each each, T
     if (!listed && sh.in_bin <= kTopkList) {
       const uint32_t range = hi - lo;
       each([&](uint32_t k) {
-        if (k - lo <= range && k != ~0u) {
+        if (k - lo <= range) {
           const int at = atomicAdd(&sh.listed, 1);
           if (at < kTopkList) sh.list[at] = k;
         }
@@ -159,8 +159,13 @@ template <int THREADS, int V, class Emit>
 __device__ __forceinline__ void topk_place(const uint32_t (&k)[V], uint32_t border, int take_equal, TopkCount& base, TopkShared& sh, Emit emit) {
   static_assert(THREADS * V <= 32768, "both counts fit a half word");
   int mine = 0;
+  uint32_t largest = k[0];
 #pragma unroll
-  for (int j = 0; j < V; ++j) mine += (k[j] > border ? 1 : 0) | (k[j] == border && border != 0u ? 0x10000 : 0);
+  for (int j = 1; j < V; ++j) largest = max(largest, k[j]);
+  if (largest >= border) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) mine += (k[j] > border ? 1 : 0) | (k[j] == border && border != 0u ? 0x10000 : 0);
+  }
   int total;
   const int before = block_exclusive<THREADS>(mine, sh, total);
   int n_gt = base.gt + (before & 0xffff), n_eq = base.eq + (before >> 16);
