@@ -387,11 +387,14 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const PageS
     for (int i = tid; i < chosen; i += kSelectThreads) { index[i] = i; table[i] = bt[i]; }
   } else {
     if (tid == 0) { sm_min = ~0u; sm_max = 0u; sm_err = 0u; sm_near = 0; sm_sure = 0; }
+    constexpr bool kIds = IN_REGS && V <= 4;   // the pages' ids too: looked up beside the scores, not after the choice
     uint32_t k[V];
+    int32_t id[kIds ? V : 1];
     auto load = [&](int i0) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int i = i0 + j;
+        if (kIds) id[kIds ? j : 0] = i < s.pages ? __ldg(bt + i) : -1;
         k[j] = i >= s.pages ? 0u : (always_taken(p, s, i) ? ~0u : order_key(__ldg(score + i)));
       }
     };
@@ -480,7 +483,7 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const PageS
         topk_place<kSelectThreads, V>(k, clear ? border : 1u, clear ? take_equal : 0, base, sh, [&](int j, int at) {
           const int i = i0 + tid * V + j;
           index[at] = i;
-          table[at] = bt[i];
+          table[at] = kIds ? id[kIds ? j : 0] : bt[i];
         });
       }
     } else {
