@@ -14,7 +14,8 @@
 // so that the loads and the first product of an item run during the sums of the one before.  Long prompts: items go back and
 // forth over the CTAs, heaviest first under a causal mask, and a key tile's query tiles are cut into shares (every
 // num_chunks-th tile), whose sums a small kernel adds in order.  Short windows (one query tile per sequence): a CTA takes
-// consecutive key tiles and keeps the query tile, which leaves the keys as the only traffic.
+// consecutive key tiles of one kv head and keeps the query tile, which leaves the keys as the only traffic; the CTAs of a
+// token's kv heads, whose rows lie side by side in memory, walk the same tiles.
 //
 // Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit; the tcgen05 product takes 512,
 // as long as its two operands take out of shared memory.  One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128, causal):
@@ -23,7 +24,7 @@
 // through a general plan of the buffers 404.  Exponentials on the FMA pipe (a degree-5 polynomial) cost more issue slots than
 // the MUFU time they save: one group of columns in eight 416 us against 404.  A quarter of the columns for four rows per thread
 // (16x256b loads) halves the shared-memory reads of the log-sum-exps and measured 399 against 404, but the registers that it
-// takes cost short windows 50 us against 43.  32 queries against 4 x 16384 keys (134 MB of keys): 38 us; a CTA per key tile 78.
+// takes cost short windows 50 us against 43.  32 queries against 4 x 16384 keys (134 MB of keys): 37 us; a CTA per key tile 78.
 #include "fa_prefill_common.cuh"
 
 namespace fa {
@@ -114,7 +115,7 @@ struct TwWalk {
     b = sequence;
     s = tw_seq(p, b);
     key_tiles = (s.len + KEYS - 1) / KEYS;
-    here = key_tiles * p.h_k * p.num_chunks;
+    here = p.resident ? key_tiles : key_tiles * p.h_k * p.num_chunks;
   }
   // Moves to the next query tile, or the next item (steps may be 0: no query sees its keys).  false: done.
   __device__ __forceinline__ bool next(const TokenWeightsParams& p) { return ++j < steps || next_item(p); }
@@ -133,9 +134,9 @@ struct TwWalk {
     }
     int i = item - base;
     int kt;
-    if (p.resident) {              // one query tile: key tiles innermost
-      hk = i / key_tiles;
-      kt = i - hk * key_tiles;
+    if (p.resident) {              // one query tile
+      kt = i;
+      hk = blockIdx.x;
       chunk = 0;
     } else {                       // key tiles outermost: heaviest first under a causal mask
       const int per = p.h_k * p.num_chunks;
@@ -153,10 +154,10 @@ struct TwWalk {
     return true;
   }
   __device__ __forceinline__ bool begin(const TokenWeightsParams& p, int total) {
-    if (p.resident) {              // a contiguous share
-      const int64_t g = gridDim.x;
-      item = static_cast<int>(total * static_cast<int64_t>(blockIdx.x) / g) - 1;
-      end = static_cast<int>(total * static_cast<int64_t>(blockIdx.x + 1) / g);
+    if (p.resident) {              // a contiguous share of the key tiles, of one kv head
+      const int64_t g = gridDim.y;
+      item = static_cast<int>(total * static_cast<int64_t>(blockIdx.y) / g) - 1;
+      end = static_cast<int>(total * static_cast<int64_t>(blockIdx.y + 1) / g);
     } else {
       round = 0;
       end = total;
@@ -252,9 +253,9 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     int total = 0;
     for (int b = lane; b < p.b; b += 32) {
       const TwSeq s = tw_seq(p, b);
-      total += (s.len + 128 * kHalvesOfKeys - 1) / (128 * kHalvesOfKeys) * p.h_k * p.num_chunks;
+      total += (s.len + 128 * kHalvesOfKeys - 1) / (128 * kHalvesOfKeys) * (p.resident ? 1 : p.h_k * p.num_chunks);
       const int n = p.cu_q[b + 1] - p.cu_q[b];
-      if (blockIdx.x == 0 && (p.seqlens[b] > p.max_len || n != s.n)) atomicOr(p.status, kRangeBit);
+      if (blockIdx.x == 0 && blockIdx.y == 0 && (p.seqlens[b] > p.max_len || n != s.n)) atomicOr(p.status, kRangeBit);
     }
     total = __reduce_add_sync(0xffffffffu, total);
     if (lane == 0) *sm_total = total;
@@ -601,10 +602,15 @@ cudaError_t launch_tw(const CUtensorMap& tq, const CUtensorMap& tk, const TokenW
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_done[dev] = true;
   }
-  const int64_t items = static_cast<int64_t>((p.max_len + p.item_keys - 1) / p.item_keys) * p.h_k * p.num_chunks * p.b;
+  const int64_t tiles = static_cast<int64_t>((p.max_len + p.item_keys - 1) / p.item_keys) * p.b;   // of keys
   const int64_t slots = 148 * (HD > 128 ? 1 : 2);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(items < slots ? items : slots));
+  if (p.resident) {
+    const int64_t shares = max(min(slots / p.h_k, tiles), int64_t{1});
+    cfg.gridDim = dim3(static_cast<unsigned>(p.h_k), static_cast<unsigned>(shares));
+  } else {
+    cfg.gridDim = dim3(static_cast<unsigned>(min(tiles * p.h_k * p.num_chunks, slots)));
+  }
   cfg.blockDim = dim3(kTwThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
