@@ -19,12 +19,12 @@
 //
 // Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit; the tcgen05 product takes 512,
 // as long as its two operands take out of shared memory.  One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128, causal):
-// 391 us, 70 % of what the MUFU units could do at the 1.7 GHz that the GPU ran at; a CTA per key tile 424 us, one CTA per SM with
+// 387 us, 70 % of what the MUFU units could do at the 1.7 GHz that the GPU ran at; a CTA per key tile 424 us, one CTA per SM with
 // 256 keys 536, eight warps per SM 436, two warps per row with half of the columns each 408, the issuing threads walking
 // through a general plan of the buffers 404.  Exponentials on the FMA pipe (a degree-5 polynomial) cost more issue slots than
 // the MUFU time they save: one group of columns in eight 416 us against 404.  A quarter of the columns for four rows per thread
 // (16x256b loads) halves the shared-memory reads of the log-sum-exps and measured 399 against 404, but the registers that it
-// takes cost short windows 50 us against 43.  32 queries against 4 x 16384 keys (134 MB of keys): 37 us; a CTA per key tile 78.
+// takes cost short windows 50 us against 43.  32 queries against 4 x 16384 keys (134 MB of keys): 34 us; a CTA per key tile 78.
 #include "fa_prefill_common.cuh"
 
 namespace fa {
@@ -120,31 +120,34 @@ struct TwWalk {
   // Moves to the next query tile, or the next item (steps may be 0: no query sees its keys).  false: done.
   __device__ __forceinline__ bool next(const TokenWeightsParams& p) { return ++j < steps || next_item(p); }
   __device__ __forceinline__ bool next_item(const TokenWeightsParams& p) {
-    if (p.resident) {
-      ++item;
-    } else {                       // back and forth, so that no CTA has the heavier item of every round
-      const int g = gridDim.x;
-      item = round * g + ((round & 1) ? g - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
-      ++round;
+    if (p.resident) {              // the next key tile, one step or none: no division, a single thread waits for each of them
+      if (++item >= end) return false;
+      k0 += KEYS;
+      while (item >= base + here) {
+        base += here;
+        enter(p, b + 1);
+        k0 = (item - base) * KEYS;
+      }
+      steps = s.tiles > 0 && !(p.causal && k0 - (s.len - s.n) >= p.tile_tokens) ? 1 : 0;
+      j = 0;
+      return true;
     }
+    // back and forth, so that no CTA has the heavier item of every round
+    const int g = gridDim.x;
+    item = round * g + ((round & 1) ? g - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+    ++round;
     if (item >= end) return false;
     while (item >= base + here) {
       base += here;
       enter(p, b + 1);
     }
+    // key tiles outermost: heaviest first under a causal mask
     int i = item - base;
-    int kt;
-    if (p.resident) {              // one query tile
-      kt = i;
-      hk = blockIdx.x;
-      chunk = 0;
-    } else {                       // key tiles outermost: heaviest first under a causal mask
-      const int per = p.h_k * p.num_chunks;
-      kt = i / per;
-      i -= kt * per;
-      hk = p.num_chunks > 1 ? i / p.num_chunks : i;
-      chunk = i - hk * p.num_chunks;
-    }
+    const int per = p.h_k * p.num_chunks;
+    const int kt = i / per;
+    i -= kt * per;
+    hk = p.num_chunks > 1 ? i / p.num_chunks : i;
+    chunk = i - hk * p.num_chunks;
     k0 = kt * KEYS;
     const int shift = s.len - s.n;                                   // query i sits at position shift + i
     first = ((p.causal && k0 > shift) ? (k0 - shift) / p.tile_tokens : 0) + chunk;
@@ -158,6 +161,10 @@ struct TwWalk {
       const int64_t g = gridDim.y;
       item = static_cast<int>(total * static_cast<int64_t>(blockIdx.y) / g) - 1;
       end = static_cast<int>(total * static_cast<int64_t>(blockIdx.y + 1) / g);
+      k0 = static_cast<int>(static_cast<uint32_t>(item) * KEYS);   // set anew in the item's sequence, unless that is the first
+      hk = blockIdx.x;
+      chunk = 0;
+      first = 0;
     } else {
       round = 0;
       end = total;
@@ -274,6 +281,8 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     if (lane == 0) {
       TwWalk<128> w{};
       int t = 0, q_key = -1, k = 0, q0 = 1, q1 = 2;
+      const int tile_boxes = 128 / p.box_rows;
+      int after_k0 = -1, after_b = -1, index = 0, row = 0;   // the key tile behind the last one: its first page and the row in it
       uint32_t loaded = 0, used = 0;
       const uint32_t q_bytes = static_cast<uint32_t>(p.tile_tokens) * p.group * 128u * T::kHalves;
       bool ok = true;
@@ -288,11 +297,23 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (p.resident) k = t & 1;
         {
           // the page ids are looked up before the wait for a buffer
-          const int nbox = min(128 / p.box_rows, (w.s.len - w.k0 + p.box_rows - 1) / p.box_rows);
+          const int nbox = w.s.len - w.k0 >= 128 ? tile_boxes : (w.s.len - w.k0 + p.box_rows - 1) / p.box_rows;
           const int32_t* bt = p.block_table + w.b * p.bt_stride;
-          int page[8];
+          if (w.k0 != after_k0 || w.b != after_b) {
+            index = w.k0 / p.page_size;
+            row = w.k0 - index * p.page_size;
+          }
+          int page[8], at[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) page[i] = i < nbox ? __ldg(bt + (w.k0 + i * p.box_rows) / p.page_size) : 0;
+          for (int i = 0; i < 8; ++i) {
+            if (i >= nbox) break;
+            page[i] = __ldg(bt + index);
+            at[i] = row;
+            row += p.box_rows;      // boxes divide pages
+            if (row >= p.page_size) { row = 0; ++index; }
+          }
+          after_k0 = w.k0 + 128;
+          after_b = w.b;
           reserve(k);
           if (!ok) break;
           const uint32_t bar = smem_u32(&full[k]);
@@ -300,10 +321,9 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (i >= nbox) break;
-            const int row = (w.k0 + i * p.box_rows) % p.page_size;
 #pragma unroll
             for (int hf = 0; hf < T::kHalves; ++hf)
-              tma_load_4d(tiles_smem + k * T::kTileBytes + hf * T::kHalfBytes + i * p.box_rows * 128, &tmap_k, bar, hf * 64, w.hk, row, page[i]);
+              tma_load_4d(tiles_smem + k * T::kTileBytes + hf * T::kHalfBytes + i * p.box_rows * 128, &tmap_k, bar, hf * 64, w.hk, at[i], page[i]);
           }
         }
         const int key = w.b * p.h_k + w.hk;
