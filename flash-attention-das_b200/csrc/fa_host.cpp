@@ -74,7 +74,10 @@ bool truth(PyObject* o) {
   if (v < 0) throw python_error();
   return v != 0;
 }
-void arguments(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "expected ", want, " arguments, got ", got); }
+void arguments(Py_ssize_t got, Py_ssize_t want) {
+  TORCH_CHECK(api.page_bounds, "bind() comes first");
+  TORCH_CHECK_TYPE(got == want, "expected ", want, " arguments, got ", got);
+}
 
 bool is_fp8(at::ScalarType t) { return t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2; }
 bool is_half(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }

@@ -3,8 +3,8 @@
 // Bounds.  lo[c] and hi[c] are the smallest and largest value of channel c among a page's keys, so for every key k of the
 // page q . k = sum_c q_c k_c <= sum_c max(q_c lo_c, q_c hi_c): a bound on the score that costs one row pair per page
 // instead of the page.  One warp per (page, kv head): 16-byte pieces of the rows, several rows in flight, packed 16-bit
-// minimum and maximum (exact: the bounds are values of the cache).  HBM-bound for a whole prompt, a few microseconds of
-// latency for the pages of one decode step.
+// minimum and maximum (exact: the bounds are values of the cache).  HBM-bound for a whole prompt (8 x 32768 tokens, 8 kv
+// heads, bf16, 0.55 GB: 82 us, the copy rate), 4 us of latency for the pages of one decode step.
 //
 // Choice.  A score kernel reads every page's bounds once and scores it in 32 bits, then one CTA per (sequence, kv head)
 // finds the border, looks again, in 64 bits, at the pages that are too near to it for 32, and writes the list.

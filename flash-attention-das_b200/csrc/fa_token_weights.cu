@@ -17,6 +17,9 @@
 // consecutive key tiles of one kv head and keeps the query tile, which leaves the keys as the only traffic; the CTAs of a
 // token's kv heads, whose rows lie side by side in memory, walk the same tiles.
 //
+// What a role's threads do from item to item is bound by instruction latency (a dozen cycles each beside 16 busy warps): the
+// walk over key tiles has no division, which took short windows from 37 to 34 us.
+//
 // Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit; the tcgen05 product takes 512,
 // as long as its two operands take out of shared memory.  One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128, causal):
 // 387 us, 70 % of what the MUFU units could do at the 1.7 GHz that the GPU ran at; a CTA per key tile 424 us, one CTA per SM with
