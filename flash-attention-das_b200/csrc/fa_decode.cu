@@ -110,7 +110,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 #ifdef FA_B200_TEST_HOOKS
         withhold = p.test_withhold && t == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
 #endif
-        issue_tile_loads<DT, HD, VT>(&tmap_k, &tmap_v, p, smem_u32(stages + s * kStageBytes), smem_u32(&full_bar[s]), sm_pages,
+        issue_tile_loads<DT, HD, VT, SC>(&tmap_k, &tmap_v, p, smem_u32(stages + s * kStageBytes), smem_u32(&full_bar[s]), sm_pages,
                                      first_page, tok_begin + t * T::kTile, tok_end, hk, withhold);
       }
     }

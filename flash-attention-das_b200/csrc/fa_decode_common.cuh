@@ -67,7 +67,8 @@ __device__ __forceinline__ void load_page_ids(const int32_t* bt, int n, int* sm_
 // full barrier is armed with the bytes that will arrive.
 // VT: the V pool is stored transposed, (num_blocks, h_k, d, page) with tokens contiguous (the reference's paged layout
 // 0, flash_attn_interface.py:2223-2227): a V tile then lands in shared memory as 128 d rows of 64 tokens.
-template <int DT, int HD, bool VT>
+// FIRST: the tile leaves L2 first (read once, and the scores that the kernel writes should stay).
+template <int DT, int HD, bool VT, bool FIRST>
 __device__ __forceinline__ void issue_tile_loads(const CUtensorMap* tmap_k, const CUtensorMap* tmap_v, const DecodeKernelParams& p,
                                                  uint32_t stage_smem, uint32_t full_bar, const int* pages, int first_page,
                                                  int tok0, int tok_end, int hk, bool withhold) {
@@ -79,6 +80,10 @@ __device__ __forceinline__ void issue_tile_loads(const CUtensorMap* tmap_k, cons
   for (int j = 0; j < boxes_per_tile; ++j) nvalid += (tok0 + j * box_tok < tok_end) ? 1 : 0;
   mbar_expect_tx(full_bar, 2u * T::kHalves * nvalid * box_bytes);
   if (withhold) return;   // failure-detection test build: the bytes announced above never arrive
+  auto load = [&](uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3) {
+    if constexpr (FIRST) tma_load_4d(dst, m, full_bar, c0, c1, c2, c3, l2_evict_first());
+    else tma_load_4d(dst, m, full_bar, c0, c1, c2, c3);
+  };
   const uint32_t kdst = stage_smem;
   const uint32_t vdst = kdst + T::kStageBytes / 2;
   for (int j = 0; j < nvalid; ++j) {
@@ -88,10 +93,10 @@ __device__ __forceinline__ void issue_tile_loads(const CUtensorMap* tmap_k, cons
     const uint32_t off = j * box_bytes;
 #pragma unroll
     for (int hf = 0; hf < T::kHalves; ++hf) {
-      tma_load_4d(kdst + hf * (T::kTile * 128) + off, tmap_k, full_bar, hf * 64, hk, row, page);
-      if constexpr (!VT) tma_load_4d(vdst + hf * (T::kTile * 128) + off, tmap_v, full_bar, hf * 64, hk, row, page);
+      load(kdst + hf * (T::kTile * 128) + off, tmap_k, hf * 64, hk, row, page);
+      if constexpr (!VT) load(vdst + hf * (T::kTile * 128) + off, tmap_v, hf * 64, hk, row, page);
     }
-    if constexpr (VT) tma_load_4d(vdst, tmap_v, full_bar, row, 0, hk, page);   // one box: 64 tokens x 128 d rows
+    if constexpr (VT) load(vdst, tmap_v, row, 0, hk, page);   // one box: 64 tokens x 128 d rows
   }
 }
 

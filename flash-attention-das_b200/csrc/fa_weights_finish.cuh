@@ -1,7 +1,8 @@
 // The weight that every key of a decode call received, from the scores that the decode kernel left behind (log2 units,
 // rows x tokens in fp32: 4 bytes per (query head, key) against 2 * d * element size of K and V per (kv head, key), which
-// stays in L2 in part) and the rows' log-sum-exp: w[t] = decay w[t] + sum_r 2^(s_rt - lse_r), rows in a fixed order.  Bound by
-// reading the scores: 16 ragged sequences of up to 32768 tokens, 16 us with the merge of the partials, after 168 of decode.
+// stays in L2 mostly, the pools' tiles being loaded to leave it first) and the rows' log-sum-exp: w[t] = decay w[t] + sum_r 2^(s_rt - lse_r), rows in a fixed order.  Bound by
+// reading the scores: 16 ragged sequences of up to 32768 tokens, 13 us with the merge of the partials, after 168 of decode
+// (16 where the tiles of K and V compete with the scores for L2).
 #pragma once
 
 #include "fa_common.cuh"
