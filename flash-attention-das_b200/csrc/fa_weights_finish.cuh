@@ -1,8 +1,8 @@
 // The weight that every key of a decode call received, from the scores that the decode kernel left behind (log2 units,
 // rows x tokens in fp32: 4 bytes per (query head, key) against 2 * d * element size of K and V per (kv head, key), which
 // stays in L2 mostly, the pools' tiles being loaded to leave it first) and the rows' log-sum-exp: w[t] = decay w[t] + sum_r 2^(s_rt - lse_r), rows in a fixed order.  Bound by
-// reading the scores: 16 ragged sequences of up to 32768 tokens, 13 us with the merge of the partials, after 168 of decode
-// (16 where the tiles of K and V compete with the scores for L2).
+// reading the scores: 16 ragged sequences of up to 32768 tokens, 11 us with the merge of the partials, after 167 of decode
+// (5 more where the tiles of K and V compete with the scores for L2, 2 more where every row looks for its query token).
 #pragma once
 
 #include "fa_common.cuh"
@@ -89,10 +89,15 @@ __device__ __forceinline__ void finish_tokens(const WeightsFinishParams& p, int 
       const float4 v = *reinterpret_cast<const float4*>(s + r * p.score_stride + tok);   // rows are padded to whole tiles
       const float lse = sm_lse[r];
       const float x[4] = {exp2f(v.x - lse), exp2f(v.y - lse), exp2f(v.z - lse), exp2f(v.w - lse)};
+      if (all) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += x[e];
+        continue;
+      }
       const int behind = p.sq - 1 - r / p.group;   // query tokens after this row's
       const int hi = p.causal ? full - behind : full, lo = p.window_left >= 0 ? full - behind - 1 - p.window_left : 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += (all || (tok + e < hi && tok + e >= lo)) ? x[e] : 0.f;
+      for (int e = 0; e < 4; ++e) sum[e] += (tok + e < hi && tok + e >= lo) ? x[e] : 0.f;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = w[e] * p.decay + sum[e];
