@@ -101,7 +101,8 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
-      const int first_page = tok_begin / p.page_size;
+      const int boxes_per_tile = T::kTile / p.box_tok;
+      int index = 0, row = tok_begin % p.page_size;
       for (int t = 0; t < n_tiles; ++t) {
         const int s = t % STAGES;
         const uint32_t ph = (t / STAGES) & 1;
@@ -111,7 +112,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         withhold = p.test_withhold && t == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
 #endif
         issue_tile_loads<DT, HD, VT, SC>(&tmap_k, &tmap_v, p, smem_u32(stages + s * kStageBytes), smem_u32(&full_bar[s]), sm_pages,
-                                     first_page, tok_begin + t * T::kTile, tok_end, hk, withhold);
+                                             index, row, boxes_per_tile, tok_begin + t * T::kTile, tok_end, hk, withhold);
       }
     }
   } else {

@@ -63,21 +63,24 @@ __device__ __forceinline__ void load_page_ids(const int32_t* bt, int n, int* sm_
 }
 
 // Producer, one thread: the TMA loads of the K/V tile that starts at token tok0 of a sequence (kTile tokens, those below
-// tok_end) into one ring stage; `pages[i]` is the physical page of the sequence's page first_page + i.  The stage's
-// full barrier is armed with the bytes that will arrive.
+// tok_end) into one ring stage; `pages[index]` is the physical page of the tile's first token and `row` its row there, both
+// moved on to the next tile (no division on the way: it would delay every refill of a stage).  The stage's full barrier is
+// armed with the bytes that will arrive.
 // VT: the V pool is stored transposed, (num_blocks, h_k, d, page) with tokens contiguous (the reference's paged layout
 // 0, flash_attn_interface.py:2223-2227): a V tile then lands in shared memory as 128 d rows of 64 tokens.
 // FIRST: the tile leaves L2 first (read once, and the scores that the kernel writes should stay).
 template <int DT, int HD, bool VT, bool FIRST>
 __device__ __forceinline__ void issue_tile_loads(const CUtensorMap* tmap_k, const CUtensorMap* tmap_v, const DecodeKernelParams& p,
-                                                 uint32_t stage_smem, uint32_t full_bar, const int* pages, int first_page,
-                                                 int tok0, int tok_end, int hk, bool withhold) {
+                                                 uint32_t stage_smem, uint32_t full_bar, const int* pages, int& index,
+                                                 int& row, int boxes_per_tile, int tok0, int tok_end, int hk, bool withhold) {
   using T = DecodeTraits<DT, HD>;
   const int box_tok = p.box_tok;
   const uint32_t box_bytes = static_cast<uint32_t>(box_tok) * 128u;  // one 128-byte column group
-  const int boxes_per_tile = T::kTile / box_tok;
-  int nvalid = 0;
-  for (int j = 0; j < boxes_per_tile; ++j) nvalid += (tok0 + j * box_tok < tok_end) ? 1 : 0;
+  int nvalid = boxes_per_tile;
+  if (tok0 + T::kTile > tok_end) {
+    nvalid = 0;
+    for (int j = 0; j < boxes_per_tile; ++j) nvalid += (tok0 + j * box_tok < tok_end) ? 1 : 0;
+  }
   mbar_expect_tx(full_bar, 2u * T::kHalves * nvalid * box_bytes);
   if (withhold) return;   // failure-detection test build: the bytes announced above never arrive
   auto load = [&](uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3) {
@@ -87,9 +90,7 @@ __device__ __forceinline__ void issue_tile_loads(const CUtensorMap* tmap_k, cons
   const uint32_t kdst = stage_smem;
   const uint32_t vdst = kdst + T::kStageBytes / 2;
   for (int j = 0; j < nvalid; ++j) {
-    const int tok = tok0 + j * box_tok;
-    const int page = pages[tok / p.page_size - first_page];
-    const int row = tok % p.page_size;
+    const int page = pages[index];
     const uint32_t off = j * box_bytes;
 #pragma unroll
     for (int hf = 0; hf < T::kHalves; ++hf) {
@@ -97,6 +98,11 @@ __device__ __forceinline__ void issue_tile_loads(const CUtensorMap* tmap_k, cons
       if constexpr (!VT) load(vdst + hf * (T::kTile * 128) + off, tmap_v, hf * 64, hk, row, page);
     }
     if constexpr (VT) load(vdst, tmap_v, row, 0, hk, page);   // one box: 64 tokens x 128 d rows
+    row += box_tok;
+    if (row >= p.page_size) {
+      row -= p.page_size;
+      ++index;
+    }
   }
 }
 
