@@ -204,11 +204,14 @@ __device__ __forceinline__ double row_score(const PageSelectParams& p, int bi, i
 // warp each, or more stages with fewer CTAs per SM measured the same or slower.
 constexpr int kScoreWarps = 4;
 constexpr int kBatch = 8;          // pages of a warp at a time: the columns of one MMA tile
-constexpr int kScoreStages = 3;    // two batches in flight per warp while one is scored
+// Two batches in flight per warp while one is scored; one above d = 128, where a batch is as large as two and shared memory
+// decides how many CTAs an SM holds.
+__host__ __device__ constexpr int score_stages(int hd) { return hd <= 128 ? 3 : 2; }
+__host__ __device__ constexpr int score_ctas(int hd) { return hd <= 128 ? 4 : hd == 192 ? 3 : 2; }   // resident on an SM
 constexpr int kMaxBatches = 32;
 // Query fragments: in registers up to d = 128 (64 of them), else in shared memory.
 __host__ __device__ constexpr bool a_in_regs(int hd) { return hd <= 128; }
-__host__ __device__ constexpr int score_smem(int hd) { return (a_in_regs(hd) ? 0 : hd / 8 * 512) + kScoreWarps * kScoreStages * kBatch * 4 * hd; }
+__host__ __device__ constexpr int score_smem(int hd) { return (a_in_regs(hd) ? 0 : hd / 8 * 512) + kScoreWarps * score_stages(hd) * kBatch * 4 * hd; }
 
 // All ones in each half whose sign bit is set.
 __device__ __forceinline__ uint32_t sign_halves(uint32_t v) {
@@ -229,6 +232,7 @@ template <int DT> __device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint3
 // the same time.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const PageSelectParams p) {
+  constexpr int kScoreStages = score_stages(HD);
   constexpr int kPieces = HD / 16;                // 64-byte pieces of a page's row pair: half of them lo, half hi
   extern __shared__ uint4 sm_dyn[];
   uint4* sm_a = sm_dyn;                           // A fragments: [2 * piece + step][lane]
@@ -542,11 +546,11 @@ cudaError_t launch_dependent(Kernel kern, dim3 grid, int threads, size_t smem, b
 
 template <int DT, int HD>
 cudaError_t launch_scores(PageSelectParams& p, cudaStream_t stream) {
-  // Batches of a warp: one while that leaves room on the GPU (four CTAs are resident on each of 148 SMs at d = 128), up to 32,
-  // which share the start-up of a CTA (lengths, page ids and queries are dependent trips to memory).
+  // Batches of a warp: one while that leaves room on the GPU (two rounds of what is resident on 148 SMs), up to 32, which share
+  // the start-up of a CTA (lengths, page ids and queries are dependent trips to memory).
   const int64_t ctas = static_cast<int64_t>((p.max_blocks + kScoreWarps * kBatch - 1) / (kScoreWarps * kBatch)) * p.h_k * p.b;
   p.batches = 1;
-  while (p.batches < kMaxBatches && ctas / (2 * p.batches) >= 148 * 8) p.batches *= 2;
+  while (p.batches < kMaxBatches && ctas / (2 * p.batches) >= 148 * 2 * score_ctas(HD)) p.batches *= 2;
   const int per_cta = kScoreWarps * kBatch * p.batches;
   const dim3 g(p.h_k, (p.max_blocks + per_cta - 1) / per_cta, p.b);
   const auto kern = page_score_kernel<DT, HD>;
