@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const Combi
 template <int NV>
 __global__ void __launch_bounds__(kCombineWarps * 32) combine_weights_kernel(const CombineKernelParams p, const WeightsFinishParams w) {
   static_assert(kCombineWarps * 32 == kFinishThreads, "one block size");
-  __shared__ float sm_lse[16];
+  __shared__ FinishRows sh;
   griddep_wait();
   griddep_launch_dependents();
   const int rows = NV > 0 ? p.rows : 0;
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_weights_kernel(con
     return;
   }
   const int i = blockIdx.x - rows, chunk = i % w.chunks, pair = i / w.chunks;
-  finish_tokens(w, chunk, pair % w.h_k, pair / w.h_k, sm_lse);
+  finish_tokens(w, chunk, pair % w.h_k, pair / w.h_k, sh);
 }
 
 }  // namespace

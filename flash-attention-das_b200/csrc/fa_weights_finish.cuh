@@ -13,9 +13,12 @@ namespace fa {
 constexpr int kFinishThreads = 128;
 constexpr int kFinishTokens = 4 * kFinishThreads;   // of a CTA: four in a row per thread
 
-// Log-sum-exp of the group's rows in log2 units -> sm_lse[16]: the merged one of an unsplit call, else from the partials
+// Of each row of the group: log-sum-exp, and the keys lo .. hi - 1 that it sees.
+struct FinishRows { float lse[16]; int lo[16], hi[16]; };
+
+// Log-sum-exp of the group's rows in log2 units: the merged one of an unsplit call, else from the partials
 // (the sink as one more term); +inf: the row has no key.  All threads; the caller synchronises.
-__device__ __forceinline__ void finish_lse(const WeightsFinishParams& p, int bi, int hk, int len, float* sm_lse) {
+__device__ __forceinline__ void finish_lse(const WeightsFinishParams& p, int bi, int hk, int len, FinishRows& sh) {
   const int rows = p.sq * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int r = warp; r < rows; r += kFinishThreads / 32) {   // row r is query token r / group, head r % group
     const int head = hk * p.group + r % p.group;
@@ -48,12 +51,17 @@ __device__ __forceinline__ void finish_lse(const WeightsFinishParams& p, int bi,
       l2 = sum > 0.f ? m2 + log2f(sum) : INFINITY;
       if (isnan(mx) || isnan(sum)) l2 = NAN;
     }
-    if (lane == 0) sm_lse[r] = l2;
+    if (lane == 0) {
+      const int behind = p.sq - 1 - r / p.group;   // query tokens after this row's
+      sh.lse[r] = l2;
+      sh.hi[r] = p.causal ? len - behind : len;
+      sh.lo[r] = p.window_left >= 0 ? len - behind - 1 - p.window_left : 0;
+    }
   }
 }
 
-// Chunks first * loops .. of kFinishTokens tokens of one (sequence, kv head).  sm_lse: 16 floats of shared memory.
-__device__ __forceinline__ void finish_tokens(const WeightsFinishParams& p, int first, int hk, int bi, float* sm_lse) {
+// Chunks first * loops .. of kFinishTokens tokens of one (sequence, kv head).  sh: shared memory.
+__device__ __forceinline__ void finish_tokens(const WeightsFinishParams& p, int first, int hk, int bi, FinishRows& sh) {
   const int rows = p.sq * p.group;
   const int full = min(p.seqlens[bi], p.max_len), len = min(full, p.capacity);
   int tok = first * p.loops * kFinishTokens;
@@ -78,26 +86,33 @@ __device__ __forceinline__ void finish_tokens(const WeightsFinishParams& p, int 
       }
     }
     if (first_pass) {
-      finish_lse(p, bi, hk, full, sm_lse);
+      finish_lse(p, bi, hk, full, sh);
       __syncthreads();
       first_pass = false;
     }
     if (tok >= len) return;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* row = s + tok;   // rows are padded to whole tiles
+    if (all) {
 #pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      const float4 v = *reinterpret_cast<const float4*>(s + r * p.score_stride + tok);   // rows are padded to whole tiles
-      const float lse = sm_lse[r];
-      const float x[4] = {exp2f(v.x - lse), exp2f(v.y - lse), exp2f(v.z - lse), exp2f(v.w - lse)};
-      if (all) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += x[e];
-        continue;
+      for (int r = 0; r < rows; ++r, row += p.score_stride) {
+        const float4 v = *reinterpret_cast<const float4*>(row);
+        const float lse = sh.lse[r];
+        sum[0] += exp2f(v.x - lse);
+        sum[1] += exp2f(v.y - lse);
+        sum[2] += exp2f(v.z - lse);
+        sum[3] += exp2f(v.w - lse);
       }
-      const int behind = p.sq - 1 - r / p.group;   // query tokens after this row's
-      const int hi = p.causal ? full - behind : full, lo = p.window_left >= 0 ? full - behind - 1 - p.window_left : 0;
+    } else {
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, row += p.score_stride) {
+        const float4 v = *reinterpret_cast<const float4*>(row);
+        const float lse = sh.lse[r];
+        const int lo = sh.lo[r], hi = sh.hi[r];
+        const float x[4] = {exp2f(v.x - lse), exp2f(v.y - lse), exp2f(v.z - lse), exp2f(v.w - lse)};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += (tok + e < hi && tok + e >= lo) ? x[e] : 0.f;
+        for (int e = 0; e < 4; ++e) sum[e] += (tok + e < hi && tok + e >= lo) ? x[e] : 0.f;
+      }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = w[e] * p.decay + sum[e];
