@@ -450,7 +450,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       TwWalk<128 * kHalvesOfKeys> w{};
       TwBuffers<kTiles> buf;
       int t = 0, q_key = -1, k_slot[2] = {0, 0}, q_slot = 0, n_half[2] = {0, 0};
-      bool ok = true, two = false;
+      bool ok = true, two = false, seen = false;   // seen: the second keys of this item have landed (a step has used them)
       bool more = w.begin(p, total);
       while (more && w.steps == 0) more = w.next(p);
       while (more && ok) {
@@ -459,6 +459,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (p.resident && load_q && q_key >= 0) buf.ends(q_slot, t - 1);
         if (w.j == 0) {
           two = w.second();
+          seen = false;
           k_slot[0] = buf.take(t + w.steps - 1);
           if (two) k_slot[1] = buf.take(t + w.steps - 1);
         }
@@ -477,9 +478,13 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           tc_fence_after();
           issue_qk<DT, HD>(tiles_smem + k_slot[half] * T::kTileBytes, tiles_smem + q_slot * T::kTileBytes, tmem_base + sb * 128);
           tc_commit(smem_u32(&s_full[sb]));
+          if (half == 1) seen = true;
         }
-        if (!ok) break;
         const bool k_done = w.j == w.steps - 1;
+        // A share of the query tiles may hold none that sees the second keys.  Their load is waited for all the same before the
+        // buffer goes back: the producer must not arm its barrier again, nor the CTA end, while the bytes are on their way.
+        if (ok && k_done && two && !seen) ok = mbar_wait(smem_u32(&full[k_slot[1]]), (buf.count(k_slot[1]) - 1) & 1, wctx);
+        if (!ok) break;
         do { more = w.next(p); } while (more && w.steps == 0);
         if (k_done) {
           tc_commit(smem_u32(&empty[k_slot[0]]));
