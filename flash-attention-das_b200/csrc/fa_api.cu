@@ -706,6 +706,7 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
       (p->q_row_stride * qes) % q_piece != 0 || p->o_batch_stride % 8 != 0 || p->o_head_stride % 8 != 0)
     return FA_B200_ERR_STRIDE;
   if (p->b == 0) return FA_B200_OK;
+  if (e_ && p->num_blocks == 0) return FA_B200_ERR_SHAPE;   // a tensor map cannot describe an empty pool
   const size_t part_bytes = decode_ws_bytes(p, pl);
   const size_t need = weights ? align256(part_bytes) + score_ws_bytes(p, pl) : part_bytes;
   if (need > 0 && (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace))) return FA_B200_ERR_WORKSPACE;
@@ -747,6 +748,7 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
   k.bt_head_stride = per_head ? e_->block_table_head_stride : 0;
   k.len_b = per_head ? p->h_k : 1;
   k.len_h = per_head ? 1 : 0;
+  k.num_blocks = e_ ? p->num_blocks : 0;
   if (weights) {
     k.scores = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + align256(part_bytes));
     k.score_stride = score_stride(pl);

@@ -24,9 +24,9 @@ namespace {
 // cache is e4m3, the queries (and the output) are 16-bit.  K is then converted to f16 in registers on its way into the
 // Q K^T product (f16 MMA; bf16 queries are converted to f16 once per CTA), V as in the all-e4m3 mode.
 // E5 (mixed mode only): the cache bytes are e5m2.
-// SC: the scaled scores are also written to p.scores, for the weight that every key receives (fa_token_weights.cu); a
-// template parameter, so that the tile loop without it stays as it is.
-template <int DT, int STAGES, bool VT, int QT = DT, int HD = 128, bool E5 = false, bool SC = false>
+// MODE: kPlain; kListed: page ids that are no pages are reported and their keys left out; kScored: that, and the scaled
+// scores are written to p.scores, for the weight that every key receives (fa_weights_finish.cuh).
+template <int DT, int STAGES, bool VT, int QT = DT, int HD = 128, bool E5 = false, int MODE = kPlain>
 __global__ void __launch_bounds__(kDecodeThreads, HD > 128 ? 1 : 2)
 decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                     const DecodeKernelParams p) {
@@ -71,7 +71,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   int len = p.seqlens[b * p.len_b + hk * p.len_h];
   if (len > p.max_len) {
     len = p.max_len;
-    if (threadIdx.x == 0 && part == 0) atomicOr(p.status, 0x10000);
+    if (threadIdx.x == 0 && part == 0) atomicOr(p.status, kRangeBit);
   }
   // Partitions past the end of this sequence have nothing to do; partition 0 of an empty sequence
   // still runs to publish "no keys" (zero output, LSE marker).
@@ -88,6 +88,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     const int first_page = tok_begin / p.page_size;
     const int n_pages = (tok_end > tok_begin) ? (tok_end - 1) / p.page_size - first_page + 1 : 0;
     load_page_ids(p.block_table + static_cast<int64_t>(b) * p.bt_stride + hk * p.bt_head_stride + first_page, n_pages, sm_pages, lane);
+    if (MODE != kPlain && lane == 0) abort_flag[2] = n_pages;
   }
   __syncthreads();
 
@@ -111,7 +112,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 #ifdef FA_B200_TEST_HOOKS
         withhold = p.test_withhold && t == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
 #endif
-        issue_tile_loads<DT, HD, VT, SC>(&tmap_k, &tmap_v, p, smem_u32(stages + s * kStageBytes), smem_u32(&full_bar[s]), sm_pages,
+        issue_tile_loads<DT, HD, VT, MODE == kScored>(&tmap_k, &tmap_v, p, smem_u32(stages + s * kStageBytes), smem_u32(&full_bar[s]), sm_pages,
                                              index, row, boxes_per_tile, tok_begin + t * T::kTile, tok_end, hk, withhold);
       }
     }
@@ -126,13 +127,21 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     if (p.q_descale) scale_log2 *= p.q_descale[b * p.qds_b + hk * p.qds_h];
     if (p.k_descale) scale_log2 *= p.k_descale[b * p.kds_b + hk * p.kds_h];
 
-    const ScoreOut so = SC ? score_out(p, b, hk, lane) : ScoreOut{};
+    // looked at here, while the first tiles are on their way, and not by the producer, which they would wait for
+    bool bad_page = false;
+    if (MODE != kPlain) {
+      bad_page = any_bad_page(sm_pages, abort_flag[2], p.num_blocks, lane);
+      if (bad_page && cw == 0 && lane == 0) atomicOr(p.status, kRangeBit);
+    }
+    const ScoreOut so = MODE == kScored ? score_out(p, b, hk, lane) : ScoreOut{};
     for (int t = 0; t < n_tiles; ++t) {
       const int s = t % STAGES;
       const uint32_t ph = (t / STAGES) & 1;
       if (!mbar_wait(smem_u32(&full_bar[s]), ph, wctx)) break;
-      consume_tile<DT, VT, QT, HD, E5, SC>(smem_u32(stages + s * kStageBytes), tok_begin + t * T::kTile, tok_end, cw, lane, qf, lim,
-                                           scale_log2, m_run, l_run, o, so);
+      int skip = 0;
+      if (bad_page) skip = bad_sub_blocks<DT, HD>(sm_pages, p.num_blocks, p.page_size, tok_begin, tok_begin + t * T::kTile, tok_end, cw);
+      consume_tile<DT, VT, QT, HD, E5, MODE>(smem_u32(stages + s * kStageBytes), tok_begin + t * T::kTile, tok_end, cw, lane, qf, lim,
+                                             scale_log2, m_run, l_run, o, so, skip);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
     }
@@ -258,14 +267,17 @@ static size_t decode_smem_bytes(int stages, int stage_bytes) {
 }
 int decode_max_pages_per_partition() { return kMaxPagesPerPartition; }
 
-template <int DT, bool VT, int QT = DT, int HD = 128, bool E5 = false, bool SC = false>
+template <int DT, bool VT, int QT = DT, int HD = 128, bool E5 = false, int MODE = kPlain>
 static cudaError_t launch_decode_dt(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeKernelParams& p,
                                     cudaStream_t stream) {
-  if constexpr (!SC && !VT)
-    if (p.scores) return launch_decode_dt<DT, VT, QT, HD, E5, true>(tk, tv, p, stream);
+  if constexpr (MODE == kPlain) {
+    if constexpr (!VT)
+      if (p.scores) return launch_decode_dt<DT, VT, QT, HD, E5, kScored>(tk, tv, p, stream);
+    if (p.num_blocks > 0) return launch_decode_dt<DT, VT, QT, HD, E5, kListed>(tk, tv, p, stream);
+  }
   // about 96 KB of tiles in flight per CTA at two CTAs per SM; one CTA per SM above d = 128
   constexpr int STAGES = HD == 64 ? 6 : (HD == 192 ? 4 : 3);
-  auto kern = decode_paged_kernel<DT, STAGES, VT, QT, HD, E5, SC>;
+  auto kern = decode_paged_kernel<DT, STAGES, VT, QT, HD, E5, MODE>;
   const size_t smem = decode_smem_bytes(STAGES, DecodeTraits<DT, HD>::kStageBytes);
   static bool attr_done[64] = {};
   int dev = 0;

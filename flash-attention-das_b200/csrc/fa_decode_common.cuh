@@ -14,6 +14,9 @@ namespace fa {
 constexpr int kConsumerWarps = 4;
 constexpr int kDecodeThreads = 32 * (1 + kConsumerWarps);
 constexpr int kMaxPagesPerPartition = 512;
+// Forms of the kernel, template parameters so that the tile loop of a plain call stays as it is: a call of
+// fa_b200_decode_budget checks the page ids, and one that accumulates token weights writes the scaled scores as well.
+constexpr int kPlain = 0, kListed = 1, kScored = 2;
 
 // HD: head dimension, 128 for every element type and 64 / 192 / 256 for the 16-bit ones.
 template <int DT, int HD = 128>
@@ -60,6 +63,27 @@ __device__ __forceinline__ void load_page_ids(const int32_t* bt, int n, int* sm_
   } else {
     for (int i = lane; i < n; i += 32) sm_pages[i] = __ldg(bt + i);
   }
+}
+
+// Whether one of the n ids in shared memory is no page of the pool, by one warp.
+__device__ __forceinline__ bool any_bad_page(const int* sm_pages, int n, int num_blocks, int lane) {
+  bool bad = false;
+  for (int i = lane; i < n; i += 32) bad = bad || static_cast<uint32_t>(sm_pages[i]) >= static_cast<uint32_t>(num_blocks);
+  return __any_sync(0xffffffffu, bad);
+}
+
+// Which of a consumer warp's 16-token sub-blocks of the tile at tok0 lie in no page (bit per sub-block; a sub-block lies in
+// one page).  Called in partitions that have such an id only.
+template <int DT, int HD>
+__device__ __forceinline__ int bad_sub_blocks(const int* sm_pages, int num_blocks, int page_size, int tok_begin, int tok0, int tok_end, int cw) {
+  using T = DecodeTraits<DT, HD>;
+  int skip = 0;
+#pragma unroll
+  for (int sb = 0; sb < T::kSub; ++sb) {
+    const int tok = tok0 + cw * T::kRowsPerWarp + sb * 16;
+    if (tok < tok_end && static_cast<uint32_t>(sm_pages[tok / page_size - tok_begin / page_size]) >= static_cast<uint32_t>(num_blocks)) skip |= 1 << sb;
+  }
+  return skip;
 }
 
 // Producer, one thread: the TMA loads of the K/V tile that starts at token tok0 of a sequence (kTile tokens, those below
@@ -190,10 +214,12 @@ __device__ __forceinline__ ScoreOut score_out(const DecodeKernelParams& p, int b
 // One consumer warp's share of one landed K/V tile (tokens tok0 .. tok0 + kTile, those below tok_end are real): the
 // warp owns kRowsPerWarp token rows of the tile and all 16 query rows; S = Q K^T with register-level MMAs, online
 // softmax in the base-2 domain, O += P V.
-template <int DT, bool VT, int QT, int HD, bool E5, bool SC, int NQ>
+// MODE: kPlain, kListed (sub-blocks named in `skip` are left out) or kScored (the scores are written too; -inf for what is
+// left out).
+template <int DT, bool VT, int QT, int HD, bool E5, int MODE, int NQ>
 __device__ __forceinline__ void consume_tile(uint32_t kbase, int tok0, int tok_end, int cw, int lane, const uint32_t (&qf)[NQ][4],
                                              const RowLimits& lim, float scale_log2, float (&m_run)[2], float (&l_run)[2],
-                                             float (&o)[DecodeTraits<DT, HD>::kNT][4], const ScoreOut so) {
+                                             float (&o)[DecodeTraits<DT, HD>::kNT][4], const ScoreOut so, int skip) {
   using T = DecodeTraits<DT, HD>;
   constexpr bool kMixed = (QT != DT);
   const int g = lane >> 2, qd = lane & 3;
@@ -217,6 +243,17 @@ __device__ __forceinline__ void consume_tile(uint32_t kbase, int tok0, int tok_e
   for (int sb = 0; sb < T::kSub; ++sb) {
     const int r0 = wrow0 + sb * 16;
     if (tok0 + r0 >= tok_end) continue;  // warp-uniform: nothing valid in this sub-block
+    if (MODE != kPlain && ((skip >> sb) & 1) != 0) {
+      if constexpr (MODE == kScored) {
+        const int tokb = tok0 + r0 + 2 * qd;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          if (so.r0) *reinterpret_cast<float2*>(so.r0 + tokb + nt * 8) = make_float2(-INFINITY, -INFINITY);
+          if (so.r1) *reinterpret_cast<float2*>(so.r1 + tokb + nt * 8) = make_float2(-INFINITY, -INFINITY);
+        }
+      }
+      continue;
+    }
     // ---- S = Q K^T for 16 tokens (two 8-token n-tiles)
     float sc[2][4];
 #pragma unroll
@@ -245,7 +282,7 @@ __device__ __forceinline__ void consume_tile(uint32_t kbase, int tok0, int tok_e
     }
     // ---- online softmax (base-2 domain), rows g and g+8
     const int tokb = tok0 + r0 + 2 * qd;
-    if constexpr (SC) {   // every token of the sub-block, also those past the end: the rows are padded to whole tiles
+    if constexpr (MODE == kScored) {   // every token of the sub-block, also those past the end: the rows are padded to whole tiles
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         if (so.r0) *reinterpret_cast<float2*>(so.r0 + tokb + nt * 8) = make_float2(sc[nt][0] * scale_log2, sc[nt][1] * scale_log2);

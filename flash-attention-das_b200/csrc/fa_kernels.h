@@ -16,6 +16,7 @@ struct DecodeKernelParams {
   const int32_t* block_table;
   int64_t bt_head_stride;   // page lists per kv head: block_table is (b, h_k, n); 0: one list per sequence
   int32_t len_b, len_h;     // length of (sequence, kv head): seqlens[b * len_b + hk * len_h]
+  int32_t num_blocks;       // pages of the pool, which the ids are checked against; 0: a plain call, whose ids are not checked
   const int32_t* seqlens;
   const float* q_descale;
   const float* k_descale;

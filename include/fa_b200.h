@@ -599,6 +599,8 @@ FA_B200_API int fa_b200_page_select(const fa_b200_page_select_params* p, void* s
  *                             exp(score - lse)
  * in fp32, keys contiguous, strides in elements; weights_out may be weights_in.  Keys at or past the length (or past
  * weights_capacity) are left as they are.  weights_out needs softmax_lse and excludes per_kv_head and o_partial_out.
+ * Page ids outside 0 .. num_blocks - 1 are reported by fa_b200_device_status() as FA_B200_ERR_DEVICE_RANGE; their keys take no
+ * part in the softmax and receive no weight.
  */
 typedef struct fa_b200_decode_budget_params {
   uint32_t struct_size;                /* sizeof(struct fa_b200_decode_budget_params) */

@@ -1,0 +1,89 @@
+"""GPU: page ids that are no pages, in the calls that attend to keys or weigh them.  Their keys are left out, as if the sequence
+did not have them, and device_status reports them.  The plain implementation gets the sequence without those pages."""
+import pytest
+import torch
+
+from oracle import cache_budget_oracle as R
+from _util import gen
+from test_cache_budget_gpu import BF, F8, HF, check_out, fa, pools, score_error  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def without(table, n, page, bad):
+    """The table and length of a sequence without the pages at `bad` (whole ones), and which of its tokens remain."""
+    keep = [j for j in range(-(-n // page)) if j not in bad]
+    seen = torch.tensor([t // page not in bad for t in range(n)], dtype=torch.bool)
+    out = torch.full_like(table, -1)
+    out[:len(keep)] = table[keep]
+    return out, int(seen.sum()), seen
+
+
+@pytest.mark.parametrize("qt,kv,d,h,h_k,sq,page,n,partition", [
+    (BF, BF, 128, 8, 2, 1, 64, 1000, None), (HF, HF, 64, 4, 4, 1, 16, 700, 256), (BF, F8, 128, 8, 2, 2, 32, 900, None),
+    (F8, F8, 128, 8, 2, 1, 64, 1500, 512), (HF, HF, 256, 8, 2, 1, 192, 1500, None), (BF, F8, 128, 4, 2, 1, 16, 333, None)])
+def test_sparse_attention_leaves_them_out(fa, monkeypatch, qt, kv, d, h, h_k, sq, page, n, partition):   # noqa: F811
+    m, cuda = fa
+    g = gen(41)
+    if partition:
+        monkeypatch.setenv("FA_B200_DECODE_PARTITION", str(partition))
+    kc, vc, bt, _, kd, vd = pools(g, [n, n - 100], h_k, page, kv, d)
+    q = torch.randn(2, sq, h, d, generator=g).to(qt)
+    last = -(-(n - 100) // page) - 1
+    table, lens = bt[:, None].expand(2, h_k, -1).clone(), torch.tensor([[n] * h_k, [n - 100] * h_k], dtype=torch.int32)
+    bads = {(0, 0): {1: -7}, (0, 1): {0: 10 ** 6, 2: kc.shape[0]}, (1, 0): {}, (1, 1): {j: -1 for j in range(last + 1)}}
+    ref_table, ref_lens = table.clone(), lens.clone()
+    for (i, x), bad in bads.items():
+        for j, v in bad.items():
+            table[i, x, j] = v
+        if len(bad) == last + 1:
+            ref_lens[i, x] = 0
+        else:
+            ref_table[i, x], ref_lens[i, x], _ = without(bt[i], int(lens[i, x]), page, bad)
+    for x in range(2, h_k):
+        ref_table[:, x], ref_lens[:, x] = bt, lens[:, x]
+    out, lse = m.sparse_attn_with_kvcache(q.cuda(), kd, vd, table.cuda(), lens.cuda(), causal=True, return_softmax_lse=True)
+    assert cuda.device_status() == 14
+    ref, ref_lse, _ = R.decode_ref(q.float(), kc.float(), vc.float(), ref_table, ref_lens, d ** -0.5)
+    check_out(out, ref, torch.nan_to_num(vc.float()).abs().amax().item(), "out")
+    tol = score_error(q, kc, d ** -0.5) + 2.0 ** -20 * 16
+    fin = ref_lse.isfinite()
+    assert torch.equal(lse.cpu().isfinite(), fin) and ((lse.cpu().double() - ref_lse)[fin].abs() <= tol).all()
+    empty = out.cpu()[1, :, h // h_k:2 * h // h_k]
+    assert (empty == 0).all() and (lse.cpu()[1, h // h_k:2 * h // h_k] == float("inf")).all()
+    m.sparse_attn_with_kvcache(q.cuda(), kd, vd, bt[:, None].expand(2, h_k, -1).contiguous().cuda(), lens.cuda())
+    assert cuda.device_status() == 0
+
+
+@pytest.mark.parametrize("qt,kv,d,h,h_k,sq,page,n,partition", [
+    (BF, BF, 128, 8, 2, 1, 64, 1000, None), (HF, HF, 128, 8, 1, 2, 16, 1500, 256), (BF, F8, 128, 8, 2, 1, 64, 900, None),
+    (F8, F8, 128, 8, 2, 4, 32, 600, None), (BF, BF, 192, 4, 2, 3, 64, 700, None)])
+def test_decode_with_weights_leaves_them_out(fa, monkeypatch, qt, kv, d, h, h_k, sq, page, n, partition):   # noqa: F811
+    m, cuda = fa
+    g = gen(42)
+    if partition:
+        monkeypatch.setenv("FA_B200_DECODE_PARTITION", str(partition))
+    kc, vc, bt, sl, kd, vd = pools(g, [n, 3 * page], h_k, page, kv, d)
+    q = torch.randn(2, sq, h, d, generator=g).to(qt)
+    bad = bt.clone()
+    bad[0, 1], bad[0, 4] = kc.shape[0], -1
+    ref_table, seen = bt.clone(), []
+    ref_lens = sl.clone()
+    ref_table[0], ref_lens[0], seen = without(bt[0], n, page, {1, 4})
+    w = torch.rand(2, h_k, bt.shape[1] * page, generator=g)
+    out, lse, got = m.flash_attn_with_kvcache_weights(q.cuda(), kd, vd, sl.cuda(), bad.cuda(), w.cuda(), causal=True,
+                                                      return_softmax_lse=True, decay=0.5)
+    assert cuda.device_status() == 14
+    ref, ref_lse, weights = R.decode_ref(q.float(), kc.float(), vc.float(), ref_table, ref_lens, d ** -0.5)
+    check_out(out, ref, torch.nan_to_num(vc.float()).abs().amax().item(), "out")
+    tol = score_error(q, kc, d ** -0.5) + 2.0 ** -20 * 16
+    assert ((lse.cpu().double() - ref_lse).abs() <= tol).all()
+    got = got.cpu().double()
+    for x in range(h_k):
+        want = 0.5 * w[0, x, :n].double()
+        want[seen] += weights[0][x]
+        assert ((got[0, x, :n] - want).abs() <= 2 * tol * want + 2.0 ** -24 * want).all()
+        assert torch.equal(got[0, x, :n][~seen], 0.5 * w[0, x, :n][~seen].double())
+        want = 0.5 * w[1, x, :3 * page].double() + weights[1][x]
+        assert ((got[1, x, :3 * page] - want).abs() <= 2 * tol * want).all()
+        assert torch.equal(got[0, x, n:], w[0, x, n:].double())
