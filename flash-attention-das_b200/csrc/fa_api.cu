@@ -1274,6 +1274,7 @@ int fa_b200_token_weights(const fa_b200_token_weights_params* p, void* stream) {
   if (p->b == 0 || max_len == 0) return FA_B200_OK;
   if (!p->cu_seqlens_q || !p->cache_seqlens || !p->block_table || !p->k_cache || !p->weights_out) return FA_B200_ERR_NULL;
   if (p->total_q > 0 && (!p->q || !p->softmax_lse)) return FA_B200_ERR_NULL;
+  if (p->num_blocks == 0) return FA_B200_ERR_SHAPE;   // a tensor map cannot describe an empty pool
   if (!aligned16(p->q) || !aligned16(p->k_cache)) return FA_B200_ERR_ALIGN;
   if (!stride_ok(p->q_row_stride, 2) || !stride_ok(p->q_head_stride, 2) || !stride_ok(p->k_block_stride, 2) ||
       !stride_ok(p->k_row_stride, 2) || !stride_ok(p->k_head_stride, 2) || p->weights_in_batch_stride < 0 ||
@@ -1307,6 +1308,7 @@ int fa_b200_token_weights(const fa_b200_token_weights_params* p, void* stream) {
   k.decay = p->decay;
   k.b = p->b; k.h = p->h; k.h_k = p->h_k; k.d = p->d;
   k.page_size = p->page_size;
+  k.num_blocks = p->num_blocks;
   k.max_len = max_len;
   k.causal = p->is_causal ? 1 : 0;
   k.scale_log2 = p->softmax_scale * kLog2e;

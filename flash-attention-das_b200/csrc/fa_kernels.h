@@ -318,7 +318,7 @@ struct TokenWeightsParams {
   int64_t win_b, win_h, wout_b, wout_h;
   int32_t capacity;
   float decay;
-  int32_t b, h, h_k, group, d, page_size, box_rows, max_len;
+  int32_t b, h, h_k, group, d, page_size, num_blocks, box_rows, max_len;
   int32_t causal;
   float scale_log2;
   int32_t tile_tokens;       // query tokens in a tile: its rows are tile_tokens x group

@@ -94,6 +94,8 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < (1 << 16) && !mbar_try_wait(bar, parity); ++i) {}
 }
 
+__device__ __forceinline__ bool page_ok(const TokenWeightsParams& p, int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks); }
+
 // The sequence's tokens and queries as every role of the kernel sees them.
 struct TwSeq { int len, q0, n, tiles; };
 __device__ __forceinline__ TwSeq tw_seq(const TokenWeightsParams& p, int b) {
@@ -236,6 +238,9 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   uint32_t* sm_tmem_base = reinterpret_cast<uint32_t*>(smem + L.misc_off);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L.misc_off + 4);
   int* sm_total = reinterpret_cast<int*>(smem + L.misc_off + 8);
+  // Not 0: the producer has met an id that is no page.  Its keys are loaded as zeros, and whoever writes sums from then on looks
+  // its key's id up and writes no sum for such a key.
+  volatile int* sm_bad = reinterpret_cast<volatile int*>(smem + L.misc_off + 12);
   const WaitCtx wctx{abort_flag, p.status};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -243,6 +248,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   griddep_launch_dependents();
   if (threadIdx.x == 32 * kProducer) {
     *abort_flag = 0;
+    *sm_bad = 0;
     for (int i = 0; i < kTiles; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
       mbar_init(smem_u32(&empty[i]), 1);
@@ -276,6 +282,10 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const uint32_t tmem_base = *sm_tmem_base;
   const int total = *sm_total;
   const uint32_t tiles_smem = smem_u32(smem);
+  auto report_page = [&] {
+    *sm_bad = 1;
+    atomicOr(p.status, kRangeBit);
+  };
 
   // Up to d = 128 (kTurns) the three tile buffers go round by rule: an item's keys take the buffer that has been out of use
   // longest, its query tiles alternate between the other two; resident: the keys alternate between 0 and 1, the query tile
@@ -307,10 +317,12 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             row = w.k0 - index * p.page_size;
           }
           int page[8], at[8];
+          bool pages_ok = true;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (i >= nbox) break;
             page[i] = __ldg(bt + index);
+            pages_ok = pages_ok && page_ok(p, page[i]);
             at[i] = row;
             row += p.box_rows;      // boxes divide pages
             if (row >= p.page_size) { row = 0; ++index; }
@@ -319,6 +331,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           after_b = w.b;
           reserve(k);
           if (!ok) break;
+          if (!pages_ok) report_page();
           const uint32_t bar = smem_u32(&full[k]);
           mbar_expect_tx(bar, static_cast<uint32_t>(nbox) * p.box_rows * 128u * T::kHalves);
 #pragma unroll
@@ -409,8 +422,10 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!ok) return;
         const uint32_t bar = smem_u32(&full[slot]);
         const int nbox = min(128 / p.box_rows, (w.s.len - k0 + p.box_rows - 1) / p.box_rows);
-        mbar_expect_tx(bar, static_cast<uint32_t>(nbox) * p.box_rows * 128u * T::kHalves);
         const int32_t* bt = p.block_table + w.b * p.bt_stride;
+        for (int i = 0; i < nbox; ++i)
+          if (!page_ok(p, __ldg(bt + (k0 + i * p.box_rows) / p.page_size))) report_page();
+        mbar_expect_tx(bar, static_cast<uint32_t>(nbox) * p.box_rows * 128u * T::kHalves);
         for (int i = 0; i < nbox; ++i) {
           const int tok = k0 + i * p.box_rows;
           const int page = bt[tok / p.page_size], row = tok % p.page_size;
@@ -580,6 +595,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         sum = now;
         if (!kTurns) ++t;
       }
+      const int bad = *sm_bad;   // set ahead of the load of the tile that it was found for, whose product has been waited for
       if (kTurns) t += w.steps;
       sum += comp;
       if (kTurns && !p.resident) {   // two buffers, so one meeting per item
@@ -590,6 +606,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         sum += s[row];
       }
       if (ok && key < w.s.len) {
+        if (bad != 0 && !page_ok(p, __ldg(p.block_table + w.b * p.bt_stride + key / p.page_size))) sum = 0.f;
         if (p.num_chunks > 1)
           p.partial[((static_cast<int64_t>(w.chunk) * p.b + w.b) * p.h_k + w.hk) * p.partial_stride + key] = sum;
         else if (key < p.capacity)

@@ -624,6 +624,7 @@ FA_B200_API int fa_b200_decode_budget(const fa_b200_decode_params* p, const fa_b
  *                             heads of the group of exp(softmax_scale * q . k_t - lse)
  * The queries of sequence b are rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] of q and the last positions of the
  * sequence; with is_causal query i of n sees the keys below len - n + i + 1.  A query whose lse is +inf gives nothing.
+ * Keys of page ids outside 0 .. num_blocks - 1 receive nothing; such ids are reported as FA_B200_ERR_DEVICE_RANGE.
  */
 typedef struct fa_b200_token_weights_params {
   uint32_t struct_size;                /* sizeof(struct fa_b200_token_weights_params) */

@@ -87,3 +87,35 @@ def test_decode_with_weights_leaves_them_out(fa, monkeypatch, qt, kv, d, h, h_k,
         want = 0.5 * w[1, x, :3 * page].double() + weights[1][x]
         assert ((got[1, x, :3 * page] - want).abs() <= 2 * tol * want).all()
         assert torch.equal(got[0, x, n:], w[0, x, n:].double())
+
+
+@pytest.mark.parametrize("dtype,d,h,h_k,page,n,queries", [
+    (BF, 128, 8, 2, 64, 600, 600), (HF, 128, 4, 2, 16, 500, 20), (BF, 256, 4, 1, 64, 700, 300), (HF, 64, 8, 1, 256, 1500, 1500),
+    (BF, 192, 8, 1, 128, 2304, 2048)])
+def test_weights_of_a_prompt_leave_them_out(fa, dtype, d, h, h_k, page, n, queries):   # noqa: F811
+    m, cuda = fa
+    g = gen(43)
+    kc, _, bt, sl, kd, _ = pools(g, [n], h_k, page, dtype, d)
+    q = torch.randn(queries, h, d, generator=g).to(dtype)
+    gone = {0, 2}
+    bad = bt.clone()
+    bad[0, 0], bad[0, 2] = -3, kc.shape[0]
+    table, left, seen = without(bt[0], n, page, gone)
+    lse = torch.empty(h, queries)
+    position = torch.arange(n)
+    w = torch.rand(1, h_k, bt.shape[1] * page, generator=g)
+    want = 0.5 * w[..., :n].double()
+    group = h // h_k
+    for x in range(h_k):
+        keys = R.rows(kc, bt[0], x, n)
+        for y in range(x * group, (x + 1) * group):
+            s = q[:, y].double() @ keys.T * d ** -0.5
+            s[(position[None, :] > torch.arange(queries)[:, None] + n - queries) | ~seen[None, :]] = -float("inf")
+            lse[y] = torch.logsumexp(s, -1).masked_fill(~(s > -float("inf")).any(-1), float("inf")).float()
+            want[0, x] += torch.exp(s - lse[y].double()[:, None]).sum(0)
+    cu = torch.tensor([0, queries], dtype=torch.int32)
+    got = m.attn_token_weights(q.cuda(), kd, lse.cuda(), cu.cuda(), queries, sl.cuda(), bad.cuda(), w.cuda(), decay=0.5).cpu()
+    assert cuda.device_status() == 14
+    tol = score_error(q, kc, d ** -0.5) + 2.0 ** -19
+    assert ((got[..., :n].double() - want).abs() <= tol * want).all()
+    assert torch.equal(got[..., :n][..., ~seen], 0.5 * w[..., :n][..., ~seen])
