@@ -387,8 +387,14 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const PageS
   int32_t* table = p.page_table + pair * p.num_pages;
   const int chosen = min(s.pages, p.num_pages);
   constexpr int kTile = V * kSelectThreads;
+  // An id that is no page is listed as it is where its page is taken all the same; sparse attention leaves its keys out.
+  auto list = [&](int at, int i, int32_t id) {
+    index[at] = i;
+    table[at] = id;
+    if (id < 0 || id >= p.num_blocks) atomicOr(p.status, kRangeBit);
+  };
   if (s.pages <= p.num_pages) {
-    for (int i = tid; i < chosen; i += kSelectThreads) { index[i] = i; table[i] = bt[i]; }
+    for (int i = tid; i < chosen; i += kSelectThreads) list(i, i, bt[i]);
   } else {
     if (tid == 0) { sm_min = ~0u; sm_max = 0u; sm_err = 0u; sm_near = 0; sm_sure = 0; }
     constexpr bool kIds = IN_REGS && V <= 4;   // the pages' ids too: looked up beside the scores, not after the choice
@@ -486,8 +492,7 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const PageS
         }
         topk_place<kSelectThreads, V>(k, clear ? border : 1u, clear ? take_equal : 0, base, sh, [&](int j, int at) {
           const int i = i0 + tid * V + j;
-          index[at] = i;
-          table[at] = kIds ? id[kIds ? j : 0] : bt[i];
+          list(at, i, kIds ? id[kIds ? j : 0] : bt[i]);
         });
       }
     } else {
@@ -517,10 +522,7 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const PageS
         const int before = n_eq + block_exclusive<kSelectThreads>(eq, sh, total);
         n_eq += total;
         const uint32_t one[1] = {i0 + tid < s.pages && (x > border64 || (eq && before < take_equal64)) ? 2u : 1u};
-        topk_place<kSelectThreads, 1>(one, 1u, 0, base, sh, [&](int, int at) {
-          index[at] = i0 + tid;
-          table[at] = bt[i0 + tid];
-        });
+        topk_place<kSelectThreads, 1>(one, 1u, 0, base, sh, [&](int, int at) { list(at, i0 + tid, bt[i0 + tid]); });
       }
     }
   }

@@ -566,7 +566,8 @@ FA_B200_API int fa_b200_page_bounds(const fa_b200_page_bounds_params* p, void* s
  * highest scores, of equal ones the lowest page (a NaN score counts as the highest).  The choice is that of the exact
  * scores: pages whose 32-bit scores lie too near the border are compared in 64 bits.  Outputs, in ascending order of
  * the page's position in the sequence and padded with -1: page_index its position, page_table the physical page;
- * seqlens_out the tokens in the chosen pages.  All of a short sequence's pages are taken.
+ * seqlens_out the tokens in the chosen pages.  All of a short sequence's pages are taken.  Ids that are no pages are
+ * reported as FA_B200_ERR_DEVICE_RANGE: such a page is listed where it is taken whatever its score, and comes last otherwise.
  */
 typedef struct fa_b200_page_select_params {
   uint32_t struct_size;                /* sizeof(struct fa_b200_page_select_params) */

@@ -119,3 +119,21 @@ def test_weights_of_a_prompt_leave_them_out(fa, dtype, d, h, h_k, page, n, queri
     tol = score_error(q, kc, d ** -0.5) + 2.0 ** -19
     assert ((got[..., :n].double() - want).abs() <= tol * want).all()
     assert torch.equal(got[..., :n][..., ~seen], 0.5 * w[..., :n][..., ~seen])
+
+
+def test_selection_reports_the_pages_that_it_lists(fa):   # noqa: F811
+    """A sequence that keeps all its pages, and pages that are taken whatever their score."""
+    m, cuda = fa
+    g = gen(44)
+    bounds = torch.randn(40, 2, 2, 128, generator=g).to(BF).cuda()
+    q = torch.randn(2, 1, 4, 128, generator=g).to(BF).cuda()
+    bt = torch.arange(40, dtype=torch.int32).reshape(2, 20)
+    for lens, at in (([128, 100], (0, 1)), ([1280, 1280], (0, 0)), ([1280, 1280], (1, 19))):
+        bad = bt.clone()
+        bad[at] = 40
+        sl = torch.tensor(lens, dtype=torch.int32).cuda()
+        m.kvcache_select_pages(q, bounds, bt.cuda(), sl, 64, 5)
+        assert cuda.device_status() == 0
+        pages, _, index = m.kvcache_select_pages(q, bounds, bad.cuda(), sl, 64, 5)
+        assert cuda.device_status() == 14
+        assert ((index[at[0]] == at[1]) == (pages[at[0]] == 40)).all()
