@@ -17,6 +17,7 @@ eager fallback — if the shared library is missing the import fails.
 import ctypes
 import importlib.util
 import os
+import threading
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -283,25 +284,23 @@ _lib.fa_b200_exchange_combine.argtypes = [ctypes.POINTER(ExchangeParams), _c_vp]
 _lib.fa_b200_exchange_combine.restype = ctypes.c_int
 _lib.fa_b200_read_stream.argtypes = [_c_vp, _c_i64, _c_vp, _c_vp]
 _lib.fa_b200_read_stream.restype = ctypes.c_int
-_lib.fa_b200_page_bounds.argtypes = [ctypes.POINTER(PageBoundsParams), _c_vp]
-_lib.fa_b200_page_bounds.restype = ctypes.c_int
-_lib.fa_b200_page_select.argtypes = [ctypes.POINTER(PageSelectParams), _c_vp]
-_lib.fa_b200_page_select.restype = ctypes.c_int
-_lib.fa_b200_page_select_workspace_bytes.argtypes = [ctypes.POINTER(PageSelectParams)]
-_lib.fa_b200_page_select_workspace_bytes.restype = ctypes.c_size_t
-_lib.fa_b200_decode_budget.argtypes = [ctypes.POINTER(DecodeParams), ctypes.POINTER(DecodeBudgetParams), _c_vp]
-_lib.fa_b200_decode_budget.restype = ctypes.c_int
-_lib.fa_b200_decode_budget_workspace_bytes.argtypes = [ctypes.POINTER(DecodeParams), ctypes.POINTER(DecodeBudgetParams)]
-_lib.fa_b200_decode_budget_workspace_bytes.restype = ctypes.c_size_t
-_lib.fa_b200_token_weights.argtypes = [ctypes.POINTER(TokenWeightsParams), _c_vp]
-_lib.fa_b200_token_weights.restype = ctypes.c_int
-_lib.fa_b200_token_weights_workspace_bytes.argtypes = [ctypes.POINTER(TokenWeightsParams)]
-_lib.fa_b200_token_weights_workspace_bytes.restype = ctypes.c_size_t
-_lib.fa_b200_kv_evict.argtypes = [ctypes.POINTER(KvEvictParams), _c_vp]
-_lib.fa_b200_kv_evict.restype = ctypes.c_int
 _lib.fa_b200_set_print_param.argtypes = [ctypes.c_int]
 _lib.fa_b200_set_print_param.restype = None
 _lib.fa_b200_last_launch_info.restype = ctypes.c_char_p
+# The bounded-cache calls (fa_host.cpp makes them; this is for C ABI callers of lib()).  FA_B200_LIB may name a library that
+# does not have them: everything else works with it.
+for _name, _restype, *_argtypes in (
+        ("fa_b200_page_bounds", ctypes.c_int, PageBoundsParams, None),
+        ("fa_b200_page_select", ctypes.c_int, PageSelectParams, None),
+        ("fa_b200_page_select_workspace_bytes", ctypes.c_size_t, PageSelectParams),
+        ("fa_b200_decode_budget", ctypes.c_int, DecodeParams, DecodeBudgetParams, None),
+        ("fa_b200_decode_budget_workspace_bytes", ctypes.c_size_t, DecodeParams, DecodeBudgetParams),
+        ("fa_b200_token_weights", ctypes.c_int, TokenWeightsParams, None),
+        ("fa_b200_token_weights_workspace_bytes", ctypes.c_size_t, TokenWeightsParams),
+        ("fa_b200_kv_evict", ctypes.c_int, KvEvictParams, None)):
+    if hasattr(_lib, _name):
+        getattr(_lib, _name).argtypes = [ctypes.POINTER(t) if t else _c_vp for t in _argtypes]
+        getattr(_lib, _name).restype = _restype
 
 
 def lib():
@@ -317,7 +316,12 @@ def set_profile_events(start: Optional["torch.cuda.Event"], stop: Optional["torc
     right before and right after its main kernel, so the dominant kernel can be timed alone."""
     global _profile_events
     _profile_events = None if start is None else (start, stop)
-    _host.set_profile_events(*((0, 0) if start is None else (start.cuda_event, stop.cuda_event)))
+    if "_host" in globals():
+        _host.set_profile_events(*_profile_handles())
+
+
+def _profile_handles():
+    return (0, 0) if _profile_events is None else tuple(e.cuda_event for e in _profile_events)
 
 
 def _own_work_counter(p, device):
@@ -1285,13 +1289,16 @@ def block_select(pooled_q, pooled_k, sim_q, sim_k, block_q, block_k, scale, cdf_
 
 
 # ------------------------------------------------------------------------------------------------
-# torch.library ops the reference's compiled extension defines on import
-# ------------------------------------------------------------------------------------------------
 # decode with a bounded KV cache
 # ------------------------------------------------------------------------------------------------
 # page_bounds, page_select, decode_budget, token_weights and kv_evict over the C ABI's functions of those names.  A decode step
 # makes several of these calls with a few microseconds of GPU work each, so their host part (checks, outputs, scratch, the
-# parameter struct) is compiled: csrc/fa_host.cpp, which lists the arguments, all positional.
+# parameter struct) is compiled: csrc/fa_host.cpp, which lists the arguments, all positional.  The module is loaded with the
+# first of these calls (below): no other entry point needs it.
+_BOUNDED = ("page_bounds", "page_select", "decode_budget", "token_weights", "kv_evict")
+_host_lock = threading.Lock()
+
+
 def _load_host():
     path = os.path.join(_HERE, "_fa_b200_host.so")
     rebuild = f"build it with `python {os.path.join(_HERE, 'build.py')} --force`"
@@ -1305,15 +1312,26 @@ def _load_host():
     spec.loader.exec_module(host)
     if torch.__version__.split("+")[0] != host.TORCH_VERSION:
         raise ImportError(f"{path} was built for torch {host.TORCH_VERSION}, this is {torch.__version__}: {rebuild}")
+    missing = [name for name in host.FUNCTIONS if not hasattr(_lib, name)]
+    if missing:
+        raise ImportError(f"{_LIB_PATH} has no bounded-cache calls ({', '.join(missing)})")
     host.bind(tuple(ctypes.cast(_lib[name], _c_vp).value for name in host.FUNCTIONS))
+    host.set_profile_events(*_profile_handles())
     return host
 
 
-_host = _load_host()
-page_bounds, page_select, decode_budget = _host.page_bounds, _host.page_select, _host.decode_budget
-token_weights, kv_evict = _host.token_weights, _host.kv_evict
+def __getattr__(name):
+    if name != "_host" and name not in _BOUNDED:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    with _host_lock:
+        if "_host" not in globals():
+            host = _load_host()
+            globals().update({n: getattr(host, n) for n in _BOUNDED}, _host=host)
+    return globals()[name]
 
 
+# ------------------------------------------------------------------------------------------------
+# torch.library ops the reference's compiled extension defines on import
 # ------------------------------------------------------------------------------------------------
 # flash_attn2_c_op::varlen_fwd and ::fwd_kvcache are C++ schemas in the reference (csrc/flash_attn_cutlass/
 # flash_api.cpp:2796-2816, TORCH_LIBRARY + TORCH_LIBRARY_IMPL); its Python interface only adds fake implementations
