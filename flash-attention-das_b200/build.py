@@ -14,6 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libfa_b200.so")
 OUT_HOST = os.path.join(HERE, "_fa_b200_host.so")
+HOST_KEY = os.path.join(HERE, "build", "_fa_b200_host.key")   # host_key() of the module that was built last
 OUT_HOOKS = os.path.join(HERE, "libfa_b200_testhooks.so")
 SOURCES = ["fa_api.cu", "fa_combine.cu", "fa_decode.cu", "fa_prefill.cu", "fa_prefill_pair.cu", "fa_prefill_dense.cu", "fa_kv_append.cu", "fa_glue.cu", "fa_block_select.cu", "fa_exchange.cu", "fa_page_select.cu", "fa_kv_evict.cu", "fa_token_weights.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -28,8 +29,24 @@ def _deps(out):
     return files
 
 
+def host_key():
+    """What the host module is built for, in full: a pre-release or vendor build of torch has a C++ ABI of its own."""
+    import torch
+    return "torch %s, Python %s" % (torch.__version__, sysconfig.get_config_var("SOABI"))
+
+
+def _built_for():
+    try:
+        with open(HOST_KEY) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def needs_build(out=OUT):
     if not os.path.exists(out):
+        return True
+    if out == OUT_HOST and _built_for() != host_key():
         return True
     t = os.path.getmtime(out)
     return any(os.path.getmtime(f) > t for f in _deps(out))
@@ -42,14 +59,18 @@ def build_host(force=False):
     import torch
     base = os.path.dirname(torch.__file__)
     part = OUT_HOST + ".%d" % os.getpid()
+    key = host_key()
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
-           "-I" + os.path.join(base, "include"), "-I" + os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           '-DFA_B200_HOST_KEY="%s"' % key, "-I" + os.path.join(base, "include"), "-I" + os.path.join(base, "include", "torch", "csrc", "api", "include"),
            "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"),
            os.path.join(CSRC, "fa_host.cpp"), "-o", part, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("g++ failed for fa_host.cpp:\n%s\n%s" % (r.stdout, r.stderr))
     os.replace(part, OUT_HOST)
+    os.makedirs(os.path.dirname(HOST_KEY), exist_ok=True)
+    with open(HOST_KEY, "w") as f:
+        f.write(key)
     return OUT_HOST
 
 

@@ -21,9 +21,12 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
-#include <torch/version.h>
 
 #include "../../include/fa_b200.h"
+
+#ifndef FA_B200_HOST_KEY
+#error "build.py names the torch and Python that this is built against"
+#endif
 
 namespace {
 
@@ -549,7 +552,7 @@ PyMODINIT_FUNC PyInit__fa_b200_host() {
     ok = name != nullptr;
     if (ok) PyTuple_SET_ITEM(names, i, name);
   }
-  ok = ok && PyModule_AddObjectRef(m, "FUNCTIONS", names) == 0 && PyModule_AddStringConstant(m, "TORCH_VERSION", TORCH_VERSION) == 0;
+  ok = ok && PyModule_AddObjectRef(m, "FUNCTIONS", names) == 0 && PyModule_AddStringConstant(m, "BUILT_FOR", FA_B200_HOST_KEY) == 0;
   Py_XDECREF(names);
   if (!ok) Py_CLEAR(m);
   return m;

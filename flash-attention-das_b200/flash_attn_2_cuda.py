@@ -17,6 +17,7 @@ eager fallback — if the shared library is missing the import fails.
 import ctypes
 import importlib.util
 import os
+import sysconfig
 import threading
 from typing import Optional, Sequence, Tuple
 
@@ -1310,8 +1311,9 @@ def _load_host():
     except ImportError as e:
         raise ImportError(f"{path} does not load with torch {torch.__version__}: {rebuild}") from e
     spec.loader.exec_module(host)
-    if torch.__version__.split("+")[0] != host.TORCH_VERSION:
-        raise ImportError(f"{path} was built for torch {host.TORCH_VERSION}, this is {torch.__version__}: {rebuild}")
+    here = f"torch {torch.__version__}, Python {sysconfig.get_config_var('SOABI')}"   # as build.py's host_key()
+    if here != host.BUILT_FOR:
+        raise ImportError(f"{path} was built for {host.BUILT_FOR}, this is {here}: {rebuild}")
     missing = [name for name in host.FUNCTIONS if not hasattr(_lib, name)]
     if missing:
         raise ImportError(f"{_LIB_PATH} has no bounded-cache calls ({', '.join(missing)})")

@@ -84,3 +84,27 @@ assert len(set(map(id, got))) == 1 and c._host.page_select is got[0] and vars(c)
 assert not hasattr(c, "no_such_call")
 """)
     assert r.returncode == 0, r.stderr
+
+
+def test_it_is_built_for_one_torch_in_full(builder, tmp_path):
+    """A pre-release differs from the release of its number, and from another pre-release; the module's own torch never does."""
+    import torch
+    import flash_attn_2_cuda
+    assert torch.__version__ in flash_attn_2_cuda._host.BUILT_FOR and flash_attn_2_cuda._host.BUILT_FOR == builder.host_key()
+    path = package(tmp_path, host=True)
+    release = torch.__version__.split("+")[0]
+    for other in (release + "a0+git1234567", release + ".dev20260101", release if "+" in torch.__version__ else release + "+vendor"):
+        r = run(path, f"import torch; torch.__version__ = {other!r}\n" + PLAIN + BOUNDED)
+        assert r.returncode == 0, r.stderr
+        assert "REFUSED" in r.stdout and other in r.stdout
+
+
+def test_a_module_of_another_torch_is_rebuilt(builder, tmp_path, monkeypatch):
+    assert not builder.needs_build(builder.OUT_HOST)
+    monkeypatch.setattr(builder, "HOST_KEY", str(tmp_path / "key"))
+    assert builder.needs_build(builder.OUT_HOST)                    # nobody knows what it was built for
+    (tmp_path / "key").write_text(builder.host_key())
+    assert not builder.needs_build(builder.OUT_HOST)
+    monkeypatch.setattr("torch.__version__", "2.99.0a0+git1234567")
+    assert "2.99.0a0+git1234567" in builder.host_key() and builder.needs_build(builder.OUT_HOST)
+    assert not builder.needs_build(builder.OUT)
