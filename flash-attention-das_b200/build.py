@@ -4,6 +4,7 @@ bounded-cache calls, against the installed torch.  Usage: python build.py [--for
 --test-hooks builds libfa_b200_testhooks.so beside it: the same sources with -DFA_B200_TEST_HOOKS (device-side waits
 give up after about a millisecond, and one entry lets a launch withhold a tile load).  Only the failure-detection
 tests load that library; the product never does."""
+import importlib.util
 import os
 import subprocess
 import sys
@@ -75,9 +76,18 @@ def build_host(force=False):
 
 
 def build(force=False, verbose=False, test_hooks=False):
-    out = OUT_HOOKS if test_hooks else OUT
+    """The library, and the host module where there is a torch to build it against (the C ABI needs none)."""
+    out = build_library(force, verbose, test_hooks)
     if not test_hooks:
-        build_host(force)
+        if importlib.util.find_spec("torch"):
+            build_host(force)
+        else:
+            sys.stderr.write("no torch: %s is not built\n" % OUT_HOST)
+    return out
+
+
+def build_library(force=False, verbose=False, test_hooks=False):
+    out = OUT_HOOKS if test_hooks else OUT
     if not force and not needs_build(out):
         return out
     objdir = os.path.join(HERE, "build", "testhooks" if test_hooks else "")

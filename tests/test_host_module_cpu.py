@@ -108,3 +108,14 @@ def test_a_module_of_another_torch_is_rebuilt(builder, tmp_path, monkeypatch):
     monkeypatch.setattr("torch.__version__", "2.99.0a0+git1234567")
     assert "2.99.0a0+git1234567" in builder.host_key() and builder.needs_build(builder.OUT_HOST)
     assert not builder.needs_build(builder.OUT)
+
+
+def test_the_library_is_built_without_torch(builder, monkeypatch, capsys):
+    """The C ABI has callers without Python packages."""
+    made = []
+    monkeypatch.setattr(builder, "build_host", lambda force=False: made.append(force))
+    monkeypatch.setattr("importlib.util.find_spec", lambda name: None)
+    assert builder.build() == builder.OUT and made == [] and "no torch" in capsys.readouterr().err
+    monkeypatch.undo()
+    monkeypatch.setattr(builder, "build_host", lambda force=False: made.append(force))
+    assert builder.build() == builder.OUT and made == [False]
