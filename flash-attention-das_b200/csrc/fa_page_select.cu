@@ -180,7 +180,7 @@ __device__ __forceinline__ double row_score(const PageSelectParams& p, int bi, i
       const int sh = 16 * (j & 1);
       const uint16_t xv = static_cast<uint16_t>((j < 2 ? x.x : x.y) >> sh);
       const uint16_t lv = static_cast<uint16_t>((j < 2 ? l.x : l.y) >> sh), hv = static_cast<uint16_t>((j < 2 ? h.x : h.y) >> sh);
-      sum = fma(to_double<DT>(xv), to_double<DT>((xv & 0x8000u) ? lv : hv), sum);
+      sum = fma(to_double<DT>(xv), to_double<DT>(xv > 0x8000u ? lv : hv), sum);   // -0 is not below 0
     }
   }
 #pragma unroll
