@@ -194,9 +194,10 @@ __device__ __forceinline__ double row_score(const PageSelectParams& p, int bi, i
 // within a k-step is free as long as both operands agree).  What is left is reading every bound once.
 //
 // Error: the products are exact and each of the 2d additions is at least a 32-bit one, in any order and rounding: at most
-// 2^-23 of a partial sum, none of which is above sum |q_c| times the largest bound.  The kernel writes that product, times
-// 2d 2^-23, per warp (with what may be flushed to zero, and infinity where it nears the end of the 32-bit range or is
-// no number); the choice below looks again in 64 bits at pages that are closer to the border.
+// 2^-23 of a partial sum, none of which is above sum |q_c| times the largest bound.  What may be flushed to zero is below
+// 2^-126: a query value (times a bound, d of them), a bound (times its query value), each product and sum, and the terms of
+// sum |q_c| itself.  The kernel writes the sum of all that per warp (and infinity where it nears the end of the 32-bit range or
+// is no number); the choice below looks again in 64 bits at pages that are closer to the border.
 //
 // 32 sequences x 131072 tokens in pages of 64, 8 kv heads, 256 MB of bounds, bf16: 51 us (5.2 TB/s; a CTA's start, which is a
 // chain of trips to memory, is what it is away from the copy rate), then 14 for the choice.  64-bit sums throughout took 148 us,
@@ -359,9 +360,10 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Page
   top = abs_max2<DT>(top, top2);
 #pragma unroll
   for (int st = 16; st > 0; st >>= 1) top = abs_max2<DT>(top, __shfl_xor_sync(0xffffffffu, top, st));
-  const float reach = q1 * Pair16<DT>::to_float(max(top & 0x7fffu, (top >> 16) & 0x7fffu)).x;   // ordered by their bits; NaN on top
+  const float most = Pair16<DT>::to_float(max(top & 0x7fffu, (top >> 16) & 0x7fffu)).x;   // ordered by their bits; NaN on top
+  const float reach = q1 * most, flushed = ((most + 4.f) * HD + q1) * 0x1p-125f;   // twice each
   if (lane == 0)   // not below 1e37: too large, or no number
-    p.errors[pair * p.err_stride + chunk * kScoreWarps + warp] = reach < 1e37f ? reach * (1.1f * 2 * HD * 0x1p-23f) + 1e-35f : INFINITY;
+    p.errors[pair * p.err_stride + chunk * kScoreWarps + warp] = reach < 1e37f ? reach * (1.1f * 2 * HD * 0x1p-23f) + flushed : INFINITY;
   cp_async_wait<0>();
 }
 
