@@ -163,8 +163,9 @@ __device__ __forceinline__ bool always_taken(const PageSelectParams& p, const Se
   return i < p.sink_pages || i >= s.pages - p.recent_pages || i >= s.open;
 }
 
-// One query row's score of a page in 64 bits by one warp; every lane returns it.  The products of 16-bit values are exact,
-// so only the sum rounds, by 2^-53: the order of the scores does not depend on the order of the sum.
+// One query row's score of a page in 64 bits by one warp; every lane returns it.  The products of 16-bit values are exact;
+// the sum rounds, in a fixed order: at most d / 32 fused multiply-adds and five additions per term, so a score is within
+// 13 * 2^-53 (d = 256) of the sum of its products' magnitudes.  Pages with equal bounds have equal scores.
 template <int DT>
 __device__ __forceinline__ double row_score(const PageSelectParams& p, int bi, int hk, int page, int r, int lane) {
   const uint16_t* lo = static_cast<const uint16_t*>(p.bounds) + (static_cast<int64_t>(page) * p.h_k + hk) * 2 * p.d;

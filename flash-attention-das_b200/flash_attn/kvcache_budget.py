@@ -68,7 +68,8 @@ def kvcache_select_pages(
     A page's score is the largest, over the queries and the heads of the group, of the sum over the channels of q_c times the
     page's largest value (q_c >= 0) or smallest value (q_c < 0): no key of the page has a larger q . k.  The first
     ``sink_pages``, the last ``recent_pages`` and the pages of the new tokens are always taken, then the highest scores, of
-    equal ones the lowest page; a NaN score counts as the highest.  The choice is exact (decided in 64 bits).
+    equal ones the lowest page; a NaN score counts as the highest.  Scores are compared as 64-bit sums in a fixed order: pages
+    with equal bounds are equal, and scores closer than 2^-48 of the sum of |q_c| |bound_c| may be taken in either order.
 
     Returns (page_table, seqlens, page_index): page_table int32 (batch, nheads_k, num_pages) the physical pages in the order of
     the sequence, -1 behind them; seqlens int32 (batch, nheads_k) the tokens in them; page_index their positions in the

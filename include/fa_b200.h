@@ -563,8 +563,9 @@ FA_B200_API int fa_b200_page_bounds(const fa_b200_page_bounds_params* p, void* s
  * over the seqlen_q query tokens and the query heads of the kv head's group, of
  *     sum_c max(q_c lo_c, q_c hi_c)    (no key of the page has a larger q . k)
  * Always taken: the first sink_pages, the last recent_pages and the pages that hold the last seqlen_q tokens; then the
- * highest scores, of equal ones the lowest page (a NaN score counts as the highest).  The choice is that of the exact
- * scores: pages whose 32-bit scores lie too near the border are compared in 64 bits.  Outputs, in ascending order of
+ * highest scores, of equal ones the lowest page (a NaN score counts as the highest).  The choice is that of 64-bit sums
+ * in a fixed order (pages whose 32-bit scores lie too near the border are compared so): equal bounds give equal scores, and
+ * scores closer than 2^-48 of the sum of |q_c| |bound_c| may be taken in either order.  Outputs, in ascending order of
  * the page's position in the sequence and padded with -1: page_index its position, page_table the physical page;
  * seqlens_out the tokens in the chosen pages.  All of a short sequence's pages are taken.  Ids that are no pages are
  * reported as FA_B200_ERR_DEVICE_RANGE: such a page is listed where it is taken whatever its score, and comes last otherwise.
