@@ -34,8 +34,8 @@ namespace fa {
 namespace {
 
 // 128-key halves of a CTA: two CTAs per SM with one up to d = 128, one CTA with two above (shared memory).  Eight warps take
-// the sums either way: with one half, two warps share 32 keys and take half of a tile's columns each (16 warps per SM keep the
-// MUFU unit busier than 8 do).
+// the sums either way: with one half, two sets of four warps take turns at the tiles, all columns of a tile each, and their sums
+// meet at the item's end (16 warps per SM keep the MUFU unit busier than 8 do).
 __host__ __device__ constexpr int tw_halves(int hd) { return hd > 128 ? 2 : 1; }
 constexpr int kTwThreads = 320;
 constexpr int kTwMaxTiles = 4;
