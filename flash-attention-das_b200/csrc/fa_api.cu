@@ -155,9 +155,12 @@ int* stream_tickets(cudaStream_t stream, int64_t count) {
 int elem_size(int dtype) { return dtype == FA_B200_E4M3 ? 1 : 2; }
 
 // 4-D tile descriptor over (d, heads, rows, batch) with a 128-byte-swizzled box of (128 bytes, box_heads, box_rows, 1).
-// Strides are in elements.  Out-of-range rows read as zero.
+// Strides are in elements.  Out-of-range rows read as zero.  A tensor map has no stride of zero: an axis that repeats the same
+// memory (an expanded tensor) is refused, an axis of one element gets any stride.
+bool repeats(int64_t n, int64_t stride) { return n > 1 && stride == 0; }
 int make_tmap(CUtensorMap* out, const void* base, int dtype, int64_t heads, int64_t rows, int64_t batch,
               int64_t head_stride, int64_t row_stride, int64_t batch_stride, int box_rows, int d = kHeadDim, int box_heads = 1) {
+  if (repeats(heads, head_stride) || repeats(rows, row_stride) || repeats(batch, batch_stride)) return FA_B200_ERR_STRIDE;
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) { set_error("cuTensorMapEncodeTiled", "driver entry point not found"); return FA_B200_ERR_CUDA; }
   const int es = elem_size(dtype);
@@ -187,6 +190,7 @@ int make_tmap(CUtensorMap* out, const void* base, int dtype, int64_t heads, int6
 // 128-byte-swizzled box of (64 tokens, 128 d rows, 1, 1) of a 16-bit type.  Strides in elements.
 int make_tmap_vt(CUtensorMap* out, const void* base, int dtype, int64_t page, int64_t heads, int64_t blocks,
                  int64_t d_stride, int64_t head_stride, int64_t block_stride) {
+  if (d_stride == 0 || repeats(heads, head_stride) || repeats(blocks, block_stride)) return FA_B200_ERR_STRIDE;
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) { set_error("cuTensorMapEncodeTiled", "driver entry point not found"); return FA_B200_ERR_CUDA; }
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(kHeadDim),
@@ -373,7 +377,7 @@ const char* fa_b200_status_string(int s) {
     case FA_B200_ERR_DTYPE: return "unsupported element type";
     case FA_B200_ERR_HEADDIM: return "head dimension must be 128 (or 64, 192, 256 with fp16 / bf16 tensors in the plain layouts)";
     case FA_B200_ERR_HEADS: return "Number of heads in key/value must divide number of heads in query (group <= 16 for decode)";
-    case FA_B200_ERR_STRIDE: return "Input tensor must have contiguous last dimension and 16-byte aligned strides";
+    case FA_B200_ERR_STRIDE: return "Input tensor must have contiguous last dimension and 16-byte aligned strides, and no stride of zero";
     case FA_B200_ERR_SHAPE: return "inconsistent or negative sizes";
     case FA_B200_ERR_PAGE: return "Paged KV cache block size must be 16, 32 or a multiple of 64";
     case FA_B200_ERR_WORKSPACE: return "workspace missing or too small";

@@ -14,8 +14,8 @@ with them the score that any key of a page can have and lists the best pages of 
 Keep less.  ``attn_token_weights`` (prompt) and ``flash_attn_with_kvcache_weights`` (decode) accumulate the attention weight
 that every cached key receives; ``kvcache_evict`` cuts every kv head to the heaviest keys and moves them together.
 
-Forward only.  Pools are (num_blocks, page_block_size, nheads_k, d) with any strides that are multiples of 16 bytes (a
-(num_blocks, nheads_k, page_block_size, d) pool is passed as its ``permute(0, 2, 1, 3)``), page_block_size 16, 32 or a
+Forward only.  Pools are (num_blocks, page_block_size, nheads_k, d) with any strides that are multiples of 16 bytes, but not
+zero (a (num_blocks, nheads_k, page_block_size, d) pool is passed as its ``permute(0, 2, 1, 3)``), page_block_size 16, 32 or a
 multiple of 64, d 128, or 64 / 192 / 256 with fp16 / bf16 pools.  Every call runs on the current stream of the tensors'
 device and can be captured into a CUDA graph; rows of padded batches have length 0.
 """

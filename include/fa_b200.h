@@ -41,7 +41,7 @@ enum {
   FA_B200_ERR_DTYPE = 2,         /* unsupported element type combination */
   FA_B200_ERR_HEADDIM = 3,       /* head dimension not 128 (64, 192, 256: fp16 / bf16 in the plain layouts only) */
   FA_B200_ERR_HEADS = 4,         /* h not a multiple of h_k, or group too large for the decode tile */
-  FA_B200_ERR_STRIDE = 5,        /* last dim not contiguous / stride not 16-byte aligned */
+  FA_B200_ERR_STRIDE = 5,        /* last dim not contiguous / stride not 16-byte aligned, or zero along an axis */
   FA_B200_ERR_SHAPE = 6,         /* negative or inconsistent sizes */
   FA_B200_ERR_PAGE = 7,          /* page size not a multiple of 16 (or of 64 above 64) */
   FA_B200_ERR_WORKSPACE = 8,     /* workspace missing or too small */

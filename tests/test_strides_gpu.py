@@ -1,0 +1,41 @@
+"""GPU: tensors whose strides the kernels cannot take are refused by the Python entry points, before any launch."""
+import pytest
+import torch
+
+from test_cache_budget_gpu import BF, fa   # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+REFUSED = "strides"
+
+
+def z(*s, t=BF):
+    return torch.zeros(*s, dtype=t, device="cuda")
+
+
+def test_expanded_keys_values_and_queries(fa):   # noqa: F811
+    m, cuda = fa
+    k, one, row = z(4, 64, 2, 128), z(4, 64, 1, 128).expand(4, 64, 2, 128), z(1, 64, 2, 128).expand(4, 64, 2, 128)
+    bt, sl, q = torch.arange(4, device="cuda", dtype=torch.int32).reshape(2, 2), torch.full((2,), 128, device="cuda", dtype=torch.int32), z(2, 1, 4, 128)
+    pages, lens = bt[:, None].expand(2, 2, 2).contiguous(), sl[:, None].expand(2, 2).contiguous()
+    w = z(2, 2, 128, t=torch.float32)
+    for bad in (one, row):
+        for kk, vv in ((bad, k), (k, bad)):
+            for call in (lambda: m.sparse_attn_with_kvcache(q, kk, vv, pages, lens),
+                         lambda: m.flash_attn_with_kvcache_weights(q, kk, vv, sl, bt, w),
+                         lambda: m.flash_attn_with_kvcache(q, kk, vv, cache_seqlens=sl, block_table=bt, causal=True)):
+                with pytest.raises(RuntimeError, match=REFUSED):
+                    call()
+        cu = torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")
+        with pytest.raises(RuntimeError, match=REFUSED):
+            m.attn_token_weights(z(6, 4, 128), bad, z(4, 6, t=torch.float32), cu, 3, sl, bt, w)
+        with pytest.raises(RuntimeError, match=REFUSED):
+            m.attn_token_weights(z(6, 1, 128).expand(6, 4, 128), k, z(4, 6, t=torch.float32), cu, 3, sl, bt, w)
+        # these read the pool by its strides
+        m.kvcache_page_bounds(bad, bt, sl)
+    x = z(2, 64, 4, 128)
+    for q3, k3, v3 in ((x, x[:1].expand(2, 64, 4, 128), x), (x, x, x[:, :, :1].expand(2, 64, 4, 128)), (z(2, 1, 4, 128).expand(2, 64, 4, 128), x, x)):
+        with pytest.raises(RuntimeError, match=REFUSED):
+            m.flash_attn_func(q3, k3, v3, causal=True)
+    torch.cuda.synchronize()
+    assert cuda.device_status() == 0
