@@ -261,6 +261,13 @@ struct DecodePlan {
   bool split;
 };
 
+// Strides of the token weights of a call: rows of the output that share memory would race.
+template <class P>
+bool weight_strides_ok(const P* p, int b, int h_k) {
+  return p->weights_in_batch_stride >= 0 && p->weights_in_head_stride >= 0 && p->weights_out_batch_stride >= 0 && p->weights_out_head_stride >= 0 &&
+         (p->weights_capacity == 0 || (!repeats(b, p->weights_out_batch_stride) && !repeats(h_k, p->weights_out_head_stride)));
+}
+
 // `budget`: a call of fa_b200_decode_budget, whose caches are short or read in part.
 DecodePlan plan_decode(const fa_b200_decode_params* p, bool budget = false) {
   DecodePlan pl{};
@@ -688,9 +695,7 @@ static int decode_paged(const fa_b200_decode_params* p, const fa_b200_decode_bud
     if (per_head || p->o_partial_out || p->v_transposed) return FA_B200_ERR_UNSUPPORTED;
     if (!p->softmax_lse) return FA_B200_ERR_NULL;
     if (e_->weights_capacity < 0) return FA_B200_ERR_SHAPE;
-    if (e_->weights_in_batch_stride < 0 || e_->weights_in_head_stride < 0 || e_->weights_out_batch_stride < 0 ||
-        e_->weights_out_head_stride < 0)
-      return FA_B200_ERR_STRIDE;
+    if (!weight_strides_ok(e_, p->b, p->h_k)) return FA_B200_ERR_STRIDE;
   }
   if (per_head && e_->block_table_head_stride < 0) return FA_B200_ERR_STRIDE;
   if (!p->q || !p->k_cache || !p->v_cache || !p->block_table || !p->cache_seqlens) return FA_B200_ERR_NULL;
@@ -1281,8 +1286,7 @@ int fa_b200_token_weights(const fa_b200_token_weights_params* p, void* stream) {
   if (p->num_blocks == 0) return FA_B200_ERR_SHAPE;   // a tensor map cannot describe an empty pool
   if (!aligned16(p->q) || !aligned16(p->k_cache)) return FA_B200_ERR_ALIGN;
   if (!stride_ok(p->q_row_stride, 2) || !stride_ok(p->q_head_stride, 2) || !stride_ok(p->k_block_stride, 2) ||
-      !stride_ok(p->k_row_stride, 2) || !stride_ok(p->k_head_stride, 2) || p->weights_in_batch_stride < 0 ||
-      p->weights_in_head_stride < 0 || p->weights_out_batch_stride < 0 || p->weights_out_head_stride < 0)
+      !stride_ok(p->k_row_stride, 2) || !stride_ok(p->k_head_stride, 2) || !weight_strides_ok(p, p->b, p->h_k))
     return FA_B200_ERR_STRIDE;
   const size_t need = fa_b200_token_weights_workspace_bytes(p);
   if (need > 0 && (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace))) return FA_B200_ERR_WORKSPACE;
@@ -1350,9 +1354,11 @@ int fa_b200_kv_evict(const fa_b200_kv_evict_params* p, void* stream) {
   const int es = fp8 ? 1 : 2;
   if (!aligned16(p->k_cache) || !aligned16(p->v_cache)) return FA_B200_ERR_ALIGN;
   if (!stride_ok(p->k_block_stride, es) || !stride_ok(p->k_row_stride, es) || !stride_ok(p->k_head_stride, es) ||
-      !stride_ok(p->v_block_stride, es) || !stride_ok(p->v_row_stride, es) || !stride_ok(p->v_head_stride, es) ||
-      p->weights_in_batch_stride < 0 || p->weights_in_head_stride < 0 || p->weights_out_batch_stride < 0 || p->weights_out_head_stride < 0)
+      !stride_ok(p->v_block_stride, es) || !stride_ok(p->v_row_stride, es) || !stride_ok(p->v_head_stride, es) || !weight_strides_ok(p, p->b, p->h_k))
     return FA_B200_ERR_STRIDE;
+  if (repeats(p->num_blocks, p->k_block_stride) || repeats(p->page_size, p->k_row_stride) || repeats(p->h_k, p->k_head_stride) ||
+      repeats(p->num_blocks, p->v_block_stride) || repeats(p->page_size, p->v_row_stride) || repeats(p->h_k, p->v_head_stride))
+    return FA_B200_ERR_STRIDE;   // rows that share memory cannot all be written
   KvEvictParams k{};
   k.status = status_ptr();
   if (!k.status) return cuda_fail("status word", cudaGetLastError());

@@ -15,6 +15,7 @@
 #include <utility>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -132,6 +133,8 @@ at::Tensor set_weights(P& p, const at::Tensor& in, const at::Tensor& out_, int64
                   what, ": token weights must be a float32 tensor (batch, nheads_k, capacity) on the cache's device with contiguous last "
                   "dimension");
   TORCH_CHECK(!in.defined() || in.size(2) == out.size(2), what, ": token_weights_out must have the shape of token_weights");
+  TORCH_CHECK(!in.defined() || !out_.defined() || at::get_overlap_status(in, out) != at::MemOverlapStatus::Partial, what,
+              ": token_weights_out must be token_weights or not overlap it");
   p.weights_in = in.defined() ? static_cast<const float*>(in.const_data_ptr()) : nullptr;
   p.weights_out = static_cast<float*>(out.mutable_data_ptr());
   const at::Tensor& i = in.defined() ? in : out;

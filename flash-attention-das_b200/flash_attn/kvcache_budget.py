@@ -135,9 +135,13 @@ def flash_attn_with_kvcache_weights(
                                       tokens and the heads of kv head hk's group
 
     token_weights: fp32 (batch, nheads_k, capacity), indexed by the position in the cache; None with ``token_weights_out``
-    given: from zero.  Without ``token_weights_out`` it is updated in place.  Entries at and behind the length are left as they
-    are.  seqlen_q x heads per kv head <= 16 (prompts: ``attn_token_weights``).  A sink (s_aux) takes part in the softmax
-    and in no key's weight.  Returns (out, token_weights_out), or (out, softmax_lse, token_weights_out)."""
+    given: from zero.  Without ``token_weights_out`` it is updated in place; an output of its own must not overlap it.  Entries at
+    and behind the length are left as they are; keys at and behind ``capacity`` are attended to and their weight is dropped.
+    seqlen_q x heads per kv head <= 16 (prompts: ``attn_token_weights``).  A sink (s_aux) takes part in the softmax and in no
+    key's weight.  Returns (out, token_weights_out), or (out, softmax_lse, token_weights_out).
+
+    Scratch: 4 bytes per (sequence, query head, query token, position that block_table covers), kept for the stream's next calls
+    for as long as the process lives; pass a table no wider than the longest sequence."""
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)
     if block_table.dim() != 2:

@@ -54,3 +54,36 @@ def test_an_axis_that_repeats_memory_has_no_tensor_map(binding):   # noqa: F811
 
     for axis in ("batch", "row", "head"):
         assert dense(**{f"q_{axis}_stride": 0}) == STRIDE, axis
+
+
+def test_rows_of_the_weights_that_share_memory(binding):   # noqa: F811
+    """Every (sequence, kv head) writes its own row."""
+    lib = binding.lib()
+    ok = dict(weights_in_batch_stride=0, weights_in_head_stride=0, weights_out_batch_stride=512, weights_out_head_stride=256, weights_capacity=256)
+    none = 1   # a null pointer that the call needs: the strides are in order
+
+    def decode_(b=2, **kw):
+        e = fill(binding.DecodeBudgetParams(), weights_out=PTR, decay=1.0, **{**ok, **kw})
+        return lib.fa_b200_decode_budget(ctypes.byref(decode(binding, b=b, q=None)), ctypes.byref(e), None)
+
+    base = dict(b=2, h_k=2, d=128, page_size=64, num_blocks=100, max_blocks_per_seq=40, dtype=1, block_table=PTR, cache_seqlens=PTR, k_cache=PTR,
+                weights_out=PTR, k_block_stride=16384, k_row_stride=256, k_head_stride=128)
+
+    def prompt(**kw):
+        p = fill(binding.TokenWeightsParams(), h=8, max_seqlen_q=10, total_q=20, q=PTR, softmax_lse=PTR, cu_seqlens_q=PTR, q_row_stride=1024,
+                 q_head_stride=128, **{**base, **ok, **kw})
+        return lib.fa_b200_token_weights(ctypes.byref(p), None)
+
+    assert decode_() == none
+    for call in (decode_, prompt):
+        assert call(weights_out_batch_stride=0) == STRIDE and call(weights_out_head_stride=0) == STRIDE
+        assert call(weights_out_batch_stride=0, b=1) != STRIDE and call(weights_out_head_stride=0, weights_capacity=0) != STRIDE
+
+    def evict(**kw):
+        p = fill(binding.KvEvictParams(), budget=100, sink_tokens=4, recent_tokens=30, v_cache=PTR, weights_in=PTR, kept_index=PTR, seqlens_out=PTR,
+                 **{**base, "v_block_stride": 16384, "v_row_stride": 256, "v_head_stride": 128, **ok, **kw})
+        return lib.fa_b200_kv_evict(ctypes.byref(p), None)
+
+    for name in ("weights_out_batch_stride", "weights_out_head_stride", "k_block_stride", "k_row_stride", "k_head_stride", "v_block_stride",
+                 "v_row_stride", "v_head_stride"):
+        assert evict(**{name: 0}) == STRIDE, name
