@@ -4,8 +4,8 @@
 // A decode step makes several of these calls with a few microseconds of GPU work each.  Argument checks, output allocation
 // and the parameter struct took 12 to 14 us of Python per call: with two kernel launches a call held the host for 17 to 20 us
 // while its kernels take 10 to 16.  Through this module it is 9 to 11 us (one launch: 4 to 5).  The module holds no state but
-// one scratch buffer per (device, stream), which grows on demand; under stream capture scratch comes fresh from the caching
-// allocator (graph-private memory).
+// one scratch buffer per (device, stream), which grows on demand up to 64 MB; more than that, and all scratch under stream
+// capture (graph-private memory), comes from the caching allocator call by call.
 #include <Python.h>
 
 #include <cmath>
@@ -155,7 +155,9 @@ void check_status(int status, const char* what) {
 }
 
 // `call(stream)` with device `index` current; p's scratch is the (device, stream)'s buffer, grown when the library refuses it as
-// too small (which it does before any launch), `size()` bytes; under capture a fresh one.
+// too small (which it does before any launch), `size()` bytes; under capture a fresh one.  Beyond kKeptBytes it goes back to the
+// caching allocator after the call (in stream order), which a call with that much to do does not notice.
+constexpr int64_t kKeptBytes = 64 << 20;
 template <class P, class Call, class Size>
 void run_with_scratch(int index, const char* what, P& p, Call call, Size size) {
   using Key = std::pair<int, void*>;
@@ -178,9 +180,11 @@ void run_with_scratch(int index, const char* what, P& p, Call call, Size size) {
   offer(kept);
   int status = call(stream);
   if (status == FA_B200_ERR_WORKSPACE) {
-    kept = at::empty({std::max<int64_t>(static_cast<int64_t>(size()), 1 << 20)}, bytes);
-    offer(kept);
+    const int64_t n = std::max<int64_t>(static_cast<int64_t>(size()), 1 << 20);
+    at::Tensor grown = at::empty({n}, bytes);
+    offer(grown);
     status = call(stream);
+    if (n <= kKeptBytes) kept = std::move(grown);
   }
   check_status(status, what);
 }

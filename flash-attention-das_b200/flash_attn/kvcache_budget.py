@@ -140,8 +140,8 @@ def flash_attn_with_kvcache_weights(
     seqlen_q x heads per kv head <= 16 (prompts: ``attn_token_weights``).  A sink (s_aux) takes part in the softmax and in no
     key's weight.  Returns (out, token_weights_out), or (out, softmax_lse, token_weights_out).
 
-    Scratch: 4 bytes per (sequence, query head, query token, position that block_table covers), kept for the stream's next calls
-    for as long as the process lives; pass a table no wider than the longest sequence."""
+    Scratch: 4 bytes per (sequence, query head, query token, position that block_table covers), so pass a table no wider than the
+    longest sequence; up to 64 MB of it are kept for the stream's next calls."""
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)
     if block_table.dim() != 2:
