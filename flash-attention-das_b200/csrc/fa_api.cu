@@ -332,9 +332,10 @@ DecodePlan plan_decode(const fa_b200_decode_params* p, bool budget = false) {
       }
     }
     // Budget calls whose grid would stay within two rounds of the 296 CTA slots: the shortest partitions that fit one round,
-    // down to four tiles, joined by the combine launch.  One sequence of 4099 tokens, 8 kv heads, bf16 (token weights): 25 us
-    // with 512 tokens merged in the kernel, 17.3 / 14.4 / 14.8 with 512 / 256 / 128 and the combine launch; 4 sequences of 4096
-    // listed tokens, fp16: 20.8 us merged in the kernel, 20.1 / 15.8 / 19.7 / 27.5 with 1024 / 512 / 256 / 128.
+    // down to four tiles, joined by the combine launch.  With pools that L2 does not hold: one sequence of 4099 tokens, 8 kv
+    // heads, bf16 (token weights) 27.7 / 18.7 / 14.0 / 12.9 / 14.4 us with 2048 / 1024 / 512 / 256 / 128 tokens; 4 sequences of
+    // 4096 listed tokens, fp16, 26.3 / 19.6 / 20.0 / 24.0 / 31.7.  Out of L2 the second reads 25.2 / 16.8 / 14.7 / 18.2 / 26.4.
+    // Merged in the kernel instead (out of L2): 25 us with 512 tokens, and 20.8.
     if (budget && rows * ((max_len + part - 1) / part) <= 2 * 296) {
       int small = 4 * pl.tile;
       while (small < max_len && rows * ((max_len + small - 1) / small) > 296) small *= 2;

@@ -329,7 +329,8 @@ __device__ __forceinline__ void consume_tile(uint32_t kbase, int tok0, int tok_e
         o[i][0] *= al0; o[i][1] *= al0; o[i][2] *= al1; o[i][3] *= al1;
       }
     }
-    // ---- O += P V
+    // ---- O += P V.  P is rounded to the 16 bits that the MMA takes, by 2^-8 (bf16) or 2^-11 (f16) of itself at most: what the
+    // output's own rounding does to it again.  The sums of P, its maxima and O stay in 32 bits.
     uint32_t pa[4];
     pa[0] = pack_p<DT>(sc[0][0], sc[0][1]);
     pa[1] = pack_p<DT>(sc[0][2], sc[0][3]);

@@ -3,7 +3,7 @@
 //
 // A decode step makes several of these calls with a few microseconds of GPU work each.  Argument checks, output allocation
 // and the parameter struct took 12 to 14 us of Python per call: with two kernel launches a call held the host for 17 to 20 us
-// while its kernels take 10 to 16.  Through this module it is 9 to 11 us (one launch: 4 to 5).  The module holds no state but
+// while its kernels take 10 to 16.  Through this module it is 9 to 12 us (one launch: 4 to 5).  The module holds no state but
 // one scratch buffer per (device, stream), which grows on demand up to 64 MB; more than that, and all scratch under stream
 // capture (graph-private memory), comes from the caching allocator call by call.
 #include <Python.h>

@@ -121,8 +121,8 @@ __host__ __device__ constexpr int move_rows(int row_bytes) {
 // and goes to, then all lanes load kMoveVectors vectors each, rows side by side, and store them.
 // blockIdx: x kv head and K / V (fastest: the heads of a token lie side by side, and their kept positions are near each
 // other), y piece of the kept rows (one CTA walks all pieces in place), z sequence.
-// 32 ragged sequences of up to 16384 tokens cut to 4096, 8 kv heads, bf16, 0.95 GB moved: 148 us (6.4 TB/s), after 26 us of
-// picking.  Picking is bound by the integer instructions of the SM that got the two longest rows; bounds of the keys for the
+// 32 ragged sequences of up to 16384 tokens cut to 4096, 8 kv heads, bf16, 0.95 GB moved: 146 us (6.5 TB/s), after 26 us of
+// picking; in place 137 (what is in its place already stays).  One sequence of 16384: 23 us with the choice, in place 44 (16 CTAs).  Picking is bound by the integer instructions of the SM that got the two longest rows; bounds of the keys for the
 // first search step, and weights taken back from their keys instead of read again, measured no better.
 __global__ void __launch_bounds__(kMoveMaxThreads) evict_move_kernel(const KvEvictParams p) {
   const int hk = blockIdx.x >> 1, bi = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -200,7 +200,7 @@ __device__ __forceinline__ double row_score(const PageSelectParams& p, int bi, i
 // sum |q_c| itself.  The kernel writes the sum of all that per warp (and infinity where it nears the end of the 32-bit range or
 // is no number); the choice below looks again in 64 bits at pages that are closer to the border.
 //
-// 32 sequences x 131072 tokens in pages of 64, 8 kv heads, 256 MB of bounds, bf16: 51 us (5.2 TB/s; a CTA's start, which is a
+// 32 sequences x 131072 tokens in pages of 64, 8 kv heads, 256 MB of bounds, bf16: 52 us (5.2 TB/s; a CTA's start, which is a
 // chain of trips to memory, is what it is away from the copy rate), then 14 for the choice.  64-bit sums throughout took 148 us,
 // 32-bit multiply-adds on the FMA pipe 84 (both bound by the instructions they issue); four heads side by side in a CTA, one
 // warp each, or more stages with fewer CTAs per SM measured the same or slower.

@@ -18,16 +18,19 @@
 // token's kv heads, whose rows lie side by side in memory, walk the same tiles.
 //
 // What a role's threads do from item to item is bound by instruction latency (a dozen cycles each beside 16 busy warps): the
-// walk over key tiles has no division, which took short windows from 37 to 34 us.
+// walk over key tiles has no division, which took short windows from 37 to 34 us (bursts, keys partly in L2).
 //
-// Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit; the tcgen05 product takes 512,
-// as long as its two operands take out of shared memory.  One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128, causal):
-// 387 us, 70 % of what the MUFU units could do at the 1.7 GHz that the GPU ran at; a CTA per key tile 424 us, one CTA per SM with
-// 256 keys 536, eight warps per SM 436, two warps per row with half of the columns each 408, the issuing threads walking
-// through a general plan of the buffers 404.  Exponentials on the FMA pipe (a degree-5 polynomial) cost more issue slots than
-// the MUFU time they save: one group of columns in eight 416 us against 404.  A quarter of the columns for four rows per thread
-// (16x256b loads) halves the shared-memory reads of the log-sum-exps and measured 399 against 404, but the registers that it
-// takes cost short windows 50 us against 43.  32 queries against 4 x 16384 keys (134 MB of keys): 34 us; a CTA per key tile 78.
+// Bound by latency beside the exponentials: 128 x 128 of them per tile take 1024 cycles of an SM's MUFU unit; the tcgen05 product
+// takes 512, as long as its two operands take out of shared memory.  One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128,
+// causal): 416 us in a series of calls (1.84 GHz under the power cap), 387 in a burst at 1.965 GHz, 59 % of what the MUFU units
+// could do; counters: MUFU pipe 67 % active, tensor pipe 33 %, issue slots 46 %, stalls on fixed latencies, on TMEM and
+// log-sum-exp loads and on shared memory.  Measured against 404 us of its time, in
+// bursts: a CTA per key tile 424 us, one CTA per SM with 256 keys 536, eight warps per SM 436, two warps per row with half of the
+// columns each 408.  Exponentials on the FMA pipe (a degree-5 polynomial) cost more issue slots than the MUFU time they save: one
+// group of columns in eight 416 us against 404.  A quarter of the columns for four rows per thread (16x256b loads) halves the
+// shared-memory reads of the log-sum-exps and measured 399 against 404, but the registers that it takes cost short windows 50 us
+// against 43.  The issuing threads' fixed walk through the buffers then took 404 to 387.  32 queries against 4 x 16384 keys (134 MB
+// of keys): 39 us with keys that L2 does not hold; a CTA per key tile 78.
 #include "fa_prefill_common.cuh"
 
 namespace fa {
