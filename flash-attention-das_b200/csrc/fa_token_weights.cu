@@ -91,8 +91,8 @@ __device__ __forceinline__ float tile_sum(uint32_t t_s, const float* neg_lse, fl
   return (a + b) + (c + d);
 }
 
-// A barrier that a copy or product in flight will still complete: waited for after an abort, with a limit, so that nothing
-// writes into memory that the CTA has given back.
+// A barrier that a copy or product in flight will still complete: waited for, with a limit, by the thread that issued it before
+// the CTA ends, so that nothing writes into memory that the CTA has given back, also where another warp has given up on a wait.
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < (1 << 16) && !mbar_try_wait(bar, parity); ++i) {}
 }
@@ -363,9 +363,8 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const int last = (w.steps & 1) ? q0 : q1, other = (w.steps & 1) ? q1 : q0, old_k = k;
         k = other; q0 = old_k; q1 = last;
       }
-      if (!ok)   // gave up: the loads issued last may still be on their way
-        for (int i = 0; i < 3; ++i)
-          if ((used >> i) & 1u) drain(smem_u32(&full[i]), ((loaded >> i) & 1u) ^ 1u);
+      for (int i = 0; i < 3; ++i)   // the loads issued last, whoever gives up on them meanwhile
+        if ((used >> i) & 1u) drain(smem_u32(&full[i]), ((loaded >> i) & 1u) ^ 1u);
     }
   } else if (kTurns && warp == kMma) {
     if (lane == 0) {
@@ -404,8 +403,7 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const int last = (w.steps & 1) ? q0 : q1, other = (w.steps & 1) ? q1 : q0, old_k = k;
         k = other; q0 = old_k; q1 = last;
       }
-      if (!ok)     // gave up: products in flight end before TMEM is freed
-        for (int i = max(0, t - 2); i < t; ++i) drain(smem_u32(&s_full[i & 1]), (i >> 1) & 1);
+      for (int i = max(0, t - 2); i < t; ++i) drain(smem_u32(&s_full[i & 1]), (i >> 1) & 1);
     }
     __syncwarp();
   } else if (warp == kProducer) {
@@ -459,9 +457,8 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!ok) break;
         ++t;
       }
-      if (!ok)   // gave up: the loads issued last may still be on their way (one reserved and not issued just runs out)
-        for (int i = 0; i < kTiles; ++i)
-          if (buf.count(i) > 0) drain(smem_u32(&full[i]), (buf.count(i) - 1) & 1);
+      for (int i = 0; i < kTiles; ++i)   // the loads issued last (one reserved and, after a wait given up, not issued just runs out)
+        if (buf.count(i) > 0) drain(smem_u32(&full[i]), (buf.count(i) - 1) & 1);
     }
   } else if (warp == kMma) {
     if (lane == 0) {
@@ -511,9 +508,8 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!p.resident || !more || w.b * p.h_k + w.hk != q_key) tc_commit(smem_u32(&empty[q_slot]));
         ++t;
       }
-      if (!ok)     // gave up: products in flight end before TMEM is freed
-        for (int half = 0; half < kHalvesOfKeys; ++half)
-          for (int i = max(0, n_half[half] - 2); i < n_half[half]; ++i) drain(smem_u32(&s_full[2 * half + (i & 1)]), (i >> 1) & 1);
+      for (int half = 0; half < kHalvesOfKeys; ++half)
+        for (int i = max(0, n_half[half] - 2); i < n_half[half]; ++i) drain(smem_u32(&s_full[2 * half + (i & 1)]), (i >> 1) & 1);
     }
     __syncwarp();
   } else {
