@@ -24,8 +24,7 @@
 // takes 512, as long as its two operands take out of shared memory.  One prompt of 8192 tokens (32 heads, 8 kv heads, d = 128,
 // causal): 416 us in a series of calls (1.84 GHz under the power cap), 387 in a burst at 1.965 GHz, 59 % of what the MUFU units
 // could do; counters: MUFU pipe 67 % active, tensor pipe 33 %, issue slots 46 %, stalls on fixed latencies, on TMEM and
-// log-sum-exp loads and on shared memory.  Measured against 404 us of its time, in
-// bursts: a CTA per key tile 424 us, one CTA per SM with 256 keys 536, eight warps per SM 436, two warps per row with half of the
+// log-sum-exp loads and on shared memory.  Measured in bursts, against 404 us then: a CTA per key tile 424 us, one CTA per SM with 256 keys 536, eight warps per SM 436, two warps per row with half of the
 // columns each 408.  Exponentials on the FMA pipe (a degree-5 polynomial) cost more issue slots than the MUFU time they save: one
 // group of columns in eight 416 us against 404.  A quarter of the columns for four rows per thread (16x256b loads) halves the
 // shared-memory reads of the log-sum-exps and measured 399 against 404, but the registers that it takes cost short windows 50 us
@@ -594,7 +593,6 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         sum = now;
         if (!kTurns) ++t;
       }
-      const int bad = *sm_bad;   // set ahead of the load of the tile that it was found for, whose product has been waited for
       if (kTurns) t += w.steps;
       sum += comp;
       if (kTurns && !p.resident) {   // two buffers, so one meeting per item
@@ -605,7 +603,8 @@ token_weights_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         sum += s[row];
       }
       if (ok && key < w.s.len) {
-        if (bad != 0 && !page_ok(p, __ldg(p.block_table + w.b * p.bt_stride + key / p.page_size))) sum = 0.f;
+        // set ahead of the load of the keys, whose product this warp has waited for, or the one that it has just met
+        if (*sm_bad != 0 && !page_ok(p, __ldg(p.block_table + w.b * p.bt_stride + key / p.page_size))) sum = 0.f;
         if (p.num_chunks > 1)
           p.partial[((static_cast<int64_t>(w.chunk) * p.b + w.b) * p.h_k + w.hk) * p.partial_stride + key] = sum;
         else if (key < p.capacity)

@@ -137,3 +137,26 @@ def test_selection_reports_the_pages_that_it_lists(fa):   # noqa: F811
         pages, _, index = m.kvcache_select_pages(q, bounds, bad.cuda(), sl, 64, 5)
         assert cuda.device_status() == 14
         assert ((index[at[0]] == at[1]) == (pages[at[0]] == 40)).all()
+
+
+def test_weights_of_a_prompt_leave_out_a_page_that_one_query_tile_sees(fa):   # noqa: F811
+    """Items of one step, which one of the two sets of summing warps takes while the other writes the sums: 40 sequences of 384 tokens,
+    a query tile of 128 tokens, the last 64 tokens of every sequence in no page."""
+    m, cuda = fa
+    g = gen(45)
+    b, n, h_k, d = 40, 384, 4, 128
+    kc, _, bt, sl, kd, _ = pools(g, [n] * b, h_k, 64, BF, d)
+    bad = bt.clone()
+    bad[:, 5] = torch.tensor([-1, kc.shape[0]] * (b // 2), dtype=torch.int32)
+    q = torch.randn(b * n, h_k, d, generator=g).to(BF)
+    lse = torch.full((h_k, b * n), 7.0)
+    cu = torch.arange(b + 1, dtype=torch.int32) * n
+    w = torch.rand(b, h_k, bt.shape[1] * 64, generator=g)
+    ref = R.token_weights_ref(q, kc, lse, cu, bt, sl, w, d ** -0.5)
+    tol = score_error(q, kc, d ** -0.5) + 2.0 ** -19
+    args = (q.cuda(), kd, lse.cuda(), cu.cuda(), n, sl.cuda(), bad.cuda())
+    for _ in range(5):
+        got = m.attn_token_weights(*args, w.cuda()).cpu()
+        assert torch.equal(got[..., 320:n], w[..., 320:n])
+        assert ((got[..., :320].double() - ref[..., :320]).abs() <= tol * ref[..., :320]).all()
+        assert cuda.device_status() == 14
